@@ -1,0 +1,223 @@
+// Host side of the paged key/value cache entries of include/fav4_bshd.h: argument checks, workspace
+// layout and launches. Nothing is allocated and the host never synchronises.
+#include <cuda_runtime.h>
+
+#include <climits>
+#include <cmath>
+#include <cstdint>
+#include <mutex>
+
+#include "fav4_bshd.h"
+#include "paged.cuh"
+
+namespace fav4 {
+namespace {
+
+constexpr int kMaxDevices = 64;
+constexpr int kMaxSms = 256;         // bound on the SMs that the workspace is laid out for
+constexpr int kPagedPerSm = 2;       // blocks of paged_attn_kernel per SM
+constexpr int kMaxGrid = kMaxSms * kPagedPerSm;
+
+bool aligned16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15) == 0; }
+bool aligned4(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 3) == 0; }
+bool stride_ok(long long s) { return s >= 0 && s % 8 == 0; }
+size_t round256(size_t n) { return (n + 255) & ~size_t(255); }
+
+// SM count, and the kernels' shared-memory limit set once per device.
+int sm_count(int* sms) {
+  static std::mutex mu;
+  static int count[kMaxDevices] = {};
+  int dev = 0;
+  cudaError_t e = cudaGetDevice(&dev);
+  if (e != cudaSuccess) return e;
+  if (dev < 0 || dev >= kMaxDevices) return cudaErrorInvalidDevice;
+  std::lock_guard<std::mutex> lock(mu);
+  if (count[dev] == 0) {
+    int n = 0;
+    e = cudaDeviceGetAttribute(&n, cudaDevAttrMultiProcessorCount, dev);
+    if (e != cudaSuccess) return e;
+    e = cudaFuncSetAttribute(paged_attn_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, kPagedSmem);
+    if (e != cudaSuccess) return e;
+    count[dev] = n < kMaxSms ? n : kMaxSms;
+  }
+  *sms = count[dev];
+  return 0;
+}
+
+bool cache_valid(const Fav4PagedCache& c) {
+  return c.k && c.v && c.page_table && c.seq_lens && aligned16(c.k) && aligned16(c.v) && aligned4(c.page_table) &&
+         aligned4(c.seq_lens) && stride_ok(c.page_stride) && stride_ok(c.token_stride) && stride_ok(c.head_stride) &&
+         c.batch > 0 && c.batch < INT_MAX && c.kv_heads > 0 && c.num_pages > 0 && c.page_size >= 16 &&
+         c.page_size % 16 == 0 && c.max_pages > 0 && c.table_stride >= 0 &&
+         static_cast<long long>(c.max_pages) * c.page_size <= INT_MAX - 1024;
+}
+
+PagedCacheView view_of(const Fav4PagedCache& c) {
+  PagedCacheView v;
+  v.k = static_cast<__nv_bfloat16*>(c.k);
+  v.v = static_cast<__nv_bfloat16*>(c.v);
+  v.page_stride = c.page_stride;
+  v.token_stride = c.token_stride;
+  v.head_stride = c.head_stride;
+  v.table = c.page_table;
+  v.table_stride = c.table_stride;
+  v.lens = c.seq_lens;
+  v.num_pages = c.num_pages;
+  v.page_size = c.page_size;
+  v.max_pages = c.max_pages;
+  v.kv_heads = c.kv_heads;
+  v.batch = c.batch;
+  return v;
+}
+
+bool append_valid(const Fav4PagedAppendArgs* a) {
+  if (!a || !cache_valid(a->cache) || a->heads <= 0 || a->heads > INT_MAX / 256 || a->cache.kv_heads > INT_MAX / 256 ||
+      a->total_q < 0 || !a->cu_seqlens_q || !aligned4(a->cu_seqlens_q) || a->rotary_dim < 0 || a->rotary_dim > 128 ||
+      a->rotary_dim % 16 || (a->interleaved != 0 && a->interleaved != 1) || !aligned4(a->offsets))
+    return false;
+  if (a->total_q == 0) return true;
+  if (!a->q || !a->k || !a->v || !a->q_out || !aligned16(a->q) || !aligned16(a->k) || !aligned16(a->v) ||
+      !aligned16(a->q_out) || !stride_ok(a->q_token_stride) || !stride_ok(a->q_head_stride) ||
+      !stride_ok(a->k_token_stride) || !stride_ok(a->k_head_stride) || !stride_ok(a->v_token_stride) ||
+      !stride_ok(a->v_head_stride))
+    return false;
+  // the tables' rows are rotary_dim / 2 floats, a multiple of 32 bytes
+  return a->rotary_dim == 0 ||
+         (a->cos_table && a->sin_table && aligned16(a->cos_table) && aligned16(a->sin_table) && a->table_rows > 0);
+}
+
+bool paged_valid(const Fav4PagedArgs* a) {
+  if (!a || !cache_valid(a->cache) || a->heads <= 0 || a->heads > INT_MAX / 256 || a->heads % a->cache.kv_heads ||
+      a->total_q < 0 || a->max_sq < 0 || a->max_sq > a->total_q || !a->cu_seqlens_q || !aligned4(a->cu_seqlens_q) ||
+      !std::isfinite(a->scale) || a->scale <= 0 || (a->prefix_pages == nullptr) != (a->prefix_len == nullptr))
+    return false;
+  if (a->prefix_pages &&
+      (!aligned4(a->prefix_pages) || !aligned4(a->prefix_len) || a->max_prefix_pages <= 0 ||
+       static_cast<long long>(a->max_prefix_pages) * a->cache.page_size > INT_MAX - 1024))
+    return false;
+  if (a->total_q == 0) return true;
+  return a->max_sq > 0 && a->q && a->o && aligned16(a->q) && aligned16(a->o) && aligned4(a->lse) &&
+         stride_ok(a->q_token_stride) && stride_ok(a->q_head_stride);
+}
+
+// Workspace: counters first (their place never changes, so that any call may follow any other), then
+// the pieces of cut units, then the prefix's result.
+struct PagedSpace {
+  size_t part_o, part_ml, prefix_o, prefix_lse, total;
+  static constexpr size_t kCounters = 2 * kMaxGrid * sizeof(uint32_t);  // own keys, prefix
+};
+PagedSpace paged_space(const Fav4PagedArgs& a) {
+  PagedSpace s;
+  s.part_o = PagedSpace::kCounters;
+  s.part_ml = s.part_o + size_t(2) * kMaxGrid * kPagedRows * 128 * sizeof(float);
+  s.prefix_o = s.part_ml + size_t(2) * kMaxGrid * kPagedRows * 2 * sizeof(float);
+  s.prefix_lse = s.prefix_o;
+  s.total = s.prefix_o;
+  if (a.prefix_pages) {
+    const size_t rows = static_cast<size_t>(a.total_q) * a.heads;
+    s.prefix_lse = s.prefix_o + round256(rows * 128 * sizeof(float));
+    s.total = s.prefix_lse + round256(rows * sizeof(float));
+  }
+  return s;
+}
+
+int launch_paged(const Fav4PagedArgs& a, int causal, uint8_t* ws, cudaStream_t stream) {
+  int sms = 0;
+  int rc = sm_count(&sms);
+  if (rc) return rc;
+  const PagedSpace sp = paged_space(a);
+  const int grid = sms * kPagedPerSm;
+  PagedParams p = {};
+  p.c = view_of(a.cache);
+  p.q = static_cast<const __nv_bfloat16*>(a.q);
+  p.q_ts = a.q_token_stride;
+  p.q_hs = a.q_head_stride;
+  p.part_o = reinterpret_cast<float*>(ws + sp.part_o);
+  p.part_ml = reinterpret_cast<float*>(ws + sp.part_ml);
+  p.arrived = reinterpret_cast<uint32_t*>(ws);
+  p.heads = a.heads;
+  p.group = a.heads / a.cache.kv_heads;
+  p.total_q = a.total_q;
+  p.scale_log2 = a.scale * 1.4426950408889634f;
+  if (a.prefix_pages) {
+    // every row of the batch against the prefix, as one sequence without a mask
+    PagedParams f = p;
+    f.c.table = a.prefix_pages;
+    f.c.lens = a.prefix_len;
+    f.c.max_pages = a.max_prefix_pages;
+    f.c.batch = 1;
+    f.max_sq = a.total_q;
+    f.o32 = reinterpret_cast<float*>(ws + sp.prefix_o);
+    f.lse = reinterpret_cast<float*>(ws + sp.prefix_lse);
+    f.arrived = p.arrived + kMaxGrid;
+    paged_attn_kernel<<<grid, kPagedWarps * 32, kPagedSmem, stream>>>(f);
+    if (cudaError_t e = cudaGetLastError(); e != cudaSuccess) return e;
+    p.add_o = f.o32;
+    p.add_lse = f.lse;
+  }
+  p.cu = a.cu_seqlens_q;
+  p.o = static_cast<__nv_bfloat16*>(a.o);
+  p.lse = a.lse;
+  p.max_sq = a.max_sq;
+  p.causal = causal;
+  paged_attn_kernel<<<grid, kPagedWarps * 32, kPagedSmem, stream>>>(p);
+  return cudaGetLastError();
+}
+
+int forward_paged(const Fav4PagedArgs* a, int causal, void* workspace, size_t bytes, cudaStream_t stream,
+                  bool prefix) {
+  if (!paged_valid(a) || (causal != 0 && causal != 1) || (a->prefix_pages != nullptr) != prefix)
+    return cudaErrorInvalidValue;
+  if (a->total_q == 0) return 0;
+  if (!workspace || (reinterpret_cast<uintptr_t>(workspace) & 255) || bytes < paged_space(*a).total)
+    return cudaErrorInvalidValue;
+  return launch_paged(*a, causal, static_cast<uint8_t*>(workspace), stream);
+}
+
+}  // namespace
+}  // namespace fav4
+
+extern "C" int fav4_bshd_paged_append(const Fav4PagedAppendArgs* a, cudaStream_t stream) {
+  if (!fav4::append_valid(a)) return cudaErrorInvalidValue;
+  if (a->total_q == 0) return 0;
+  fav4::AppendParams p;
+  p.c = fav4::view_of(a->cache);
+  p.q = static_cast<const __nv_bfloat16*>(a->q);
+  p.k = static_cast<const __nv_bfloat16*>(a->k);
+  p.v = static_cast<const __nv_bfloat16*>(a->v);
+  p.q_out = static_cast<__nv_bfloat16*>(a->q_out);
+  p.cu = a->cu_seqlens_q;
+  p.cos_t = a->cos_table;
+  p.sin_t = a->sin_table;
+  p.offsets = a->offsets;
+  p.q_ts = a->q_token_stride;
+  p.q_hs = a->q_head_stride;
+  p.k_ts = a->k_token_stride;
+  p.k_hs = a->k_head_stride;
+  p.v_ts = a->v_token_stride;
+  p.v_hs = a->v_head_stride;
+  p.heads = a->heads;
+  p.total_q = a->total_q;
+  p.rotary = a->rotary_dim;
+  p.table_rows = a->table_rows;
+  const long long per_token = (a->heads + 2ll * a->cache.kv_heads + fav4::kAppendRows - 1) / fav4::kAppendRows;
+  const long long blocks = (a->total_q * per_token + 7) / 8;
+  if (blocks > INT_MAX) return cudaErrorInvalidValue;
+  auto kernel = a->interleaved ? fav4::paged_append_kernel<true> : fav4::paged_append_kernel<false>;
+  kernel<<<static_cast<unsigned>(blocks), 256, 0, stream>>>(p);
+  return cudaGetLastError();
+}
+
+extern "C" size_t fav4_bshd_paged_workspace_bytes(const Fav4PagedArgs* a) {
+  return fav4::paged_valid(a) ? fav4::paged_space(*a).total : 0;
+}
+
+extern "C" int fav4_bshd_forward_paged(const Fav4PagedArgs* a, int causal, void* workspace, size_t workspace_bytes,
+                                       cudaStream_t stream) {
+  return fav4::forward_paged(a, causal, workspace, workspace_bytes, stream, false);
+}
+
+extern "C" int fav4_bshd_forward_shared_prefix(const Fav4PagedArgs* a, int causal, void* workspace,
+                                               size_t workspace_bytes, cudaStream_t stream) {
+  return fav4::forward_paged(a, causal, workspace, workspace_bytes, stream, true);
+}

@@ -1,0 +1,616 @@
+// Paged key/value cache: the kernels around its pages (no reference counterpart; the reference has
+// no cache).
+//
+// A cache is two BF16 arrays of num_pages pages of page_size keys. Key s of sequence b lives in slot
+// s % page_size of page table[b][s / page_size]. Queries are packed rows: sequence b owns
+// [cu[b], cu[b+1]), and its row i stands at position len_b - sq_b + i, so its last row is its newest
+// key.
+#pragma once
+#include <cuda_bf16.h>
+#include <cstdint>
+#include "sm100.cuh"
+
+namespace fav4 {
+
+struct PagedCacheView {
+  __nv_bfloat16 *k, *v;
+  int64_t page_stride, token_stride, head_stride;  // elements
+  const int* table;                                // [batch][table_stride]
+  int64_t table_stride;
+  const int* lens;  // keys per sequence, this step's included
+  int num_pages, page_size, max_pages, kv_heads, batch;
+};
+
+// Rows, keys and offsets of one sequence, clamped so that malformed offsets, lengths or page numbers
+// can give wrong rows but no access outside the tensors.
+struct SeqView {
+  int q0, sq, len;
+};
+
+__device__ __forceinline__ SeqView seq_view(const PagedCacheView& c, const int* cu, int total_q, int max_sq, int b) {
+  SeqView s;
+  if (cu != nullptr) {
+    s.q0 = min(max(__ldg(cu + b), 0), total_q);
+    s.sq = min(min(max(__ldg(cu + b + 1), s.q0), total_q) - s.q0, max_sq);
+  } else {  // one sequence of all rows
+    s.q0 = 0;
+    s.sq = total_q;
+  }
+  const int64_t cap = static_cast<int64_t>(c.max_pages) * c.page_size;
+  s.len = static_cast<int>(min(static_cast<int64_t>(max(__ldg(c.lens + b), 0)), cap));
+  return s;
+}
+
+// ------------------------------------------------------------------------------------------------
+// Append: q' = R(pos) q, and k' = R(pos) k, v into their slots.
+//
+// R turns each pair (x_i, y_i), i < rotary/2, by the angle of row pos of the cos / sin tables:
+// (x cos - y sin, y cos + x sin). Pairs are (i, i + rotary/2), or (2i, 2i + 1) when interleaved;
+// elements from `rotary` on pass unchanged. The arithmetic is FP32 and each result is rounded once.
+//
+// Bandwidth: every row (one head of one token, 256 bytes) is read once and written once. A warp takes
+// 8 rows of one token, 8 lanes per row; a lane holds the two 16-byte pieces that contain 8 whole
+// pairs, and because both pairings put pairs 8s..8s+7 into lane s, the lane's slice of cos / sin is
+// the same 32 bytes either way and is loaded once for its rows.
+// ------------------------------------------------------------------------------------------------
+struct AppendParams {
+  PagedCacheView c;
+  const __nv_bfloat16 *q, *k, *v;
+  __nv_bfloat16* q_out;  // [total_q, heads, 128]
+  const int* cu;
+  const float *cos_t, *sin_t;  // [table_rows, rotary/2]
+  const int* offsets;          // rotation position = cache position + offsets[b]; may be null
+  int64_t q_ts, q_hs, k_ts, k_hs, v_ts, v_hs;  // strides in elements
+  int heads, total_q, rotary, table_rows;
+};
+
+// The sequence of packed row t: the number of b with cu[b+1] <= t. 32 probes per step.
+__device__ __forceinline__ int find_sequence(const int* cu, int batch, int t, int lane) {
+  int lo = 0, hi = batch;
+  while (lo < hi) {
+    const int step = (hi - lo + 31) / 32;
+    const int64_t i = lo + static_cast<int64_t>(lane) * step + step - 1;
+    const bool before = i < hi && __ldg(cu + i + 1) <= t;
+    lo += __popc(__ballot_sync(0xffffffffu, before)) * step;
+    hi = min(hi, lo + step - 1);
+  }
+  return lo;
+}
+
+__device__ __forceinline__ void rotate_pairs(uint32_t& a, uint32_t& b, float2 c, float2 s) {
+  // two pairs: (a.lo, b.lo) by (c.x, s.x) and (a.hi, b.hi) by (c.y, s.y)
+  const float2 x = __bfloat1622float2(*reinterpret_cast<__nv_bfloat162*>(&a));
+  const float2 y = __bfloat1622float2(*reinterpret_cast<__nv_bfloat162*>(&b));
+  a = pack_bf16x2(x.x * c.x - y.x * s.x, x.y * c.y - y.y * s.y);
+  b = pack_bf16x2(y.x * c.x + x.x * s.x, y.y * c.y + x.y * s.y);
+}
+
+constexpr int kAppendRows = 8;  // rows of one token per warp
+
+template <bool Interleaved>
+__global__ void __launch_bounds__(256) paged_append_kernel(const __grid_constant__ AppendParams p) {
+  const int lane = threadIdx.x % 32;
+  const int hk = p.c.kv_heads, rows = p.heads + 2 * hk;
+  const int per_token = (rows + kAppendRows - 1) / kAppendRows;
+  const int64_t item = (static_cast<int64_t>(blockIdx.x) * blockDim.x + threadIdx.x) / 32;
+  if (item >= static_cast<int64_t>(p.total_q) * per_token) return;
+  const int t = static_cast<int>(item / per_token);
+  const int r0 = static_cast<int>(item - static_cast<int64_t>(t) * per_token) * kAppendRows;
+  const int slot = lane % 8;  // pairs 8 slot .. 8 slot + 7
+  const bool turned = slot < p.rotary / 16;
+  // 16-byte pieces of this lane within a row
+  int pa, pb;
+  if (Interleaved) {
+    pa = 2 * slot;
+    pb = pa + 1;
+  } else if (turned) {
+    pa = slot;
+    pb = slot + p.rotary / 16;
+  } else {
+    pa = 2 * slot;  // past the rotated elements: rotary/8 + 2 (slot - rotary/16)
+    pb = pa + 1;
+  }
+  // the rows do not depend on the sequence: their loads go out first
+  uint4 a[2], b[2];
+#pragma unroll
+  for (int u = 0; u < 2; ++u) {
+    const int r = r0 + u * 4 + lane / 8;
+    const __nv_bfloat16* src = nullptr;
+    if (r < p.heads) src = p.q + t * p.q_ts + r * p.q_hs;
+    else if (r < p.heads + hk) src = p.k + t * p.k_ts + (r - p.heads) * p.k_hs;
+    else if (r < rows) src = p.v + t * p.v_ts + (r - p.heads - hk) * p.v_hs;
+    if (src != nullptr) {
+      a[u] = *reinterpret_cast<const uint4*>(src + pa * 8);
+      b[u] = *reinterpret_cast<const uint4*>(src + pb * 8);
+    }
+  }
+  const int seq = find_sequence(p.cu, p.c.batch, t, lane);
+  if (seq >= p.c.batch) return;  // a row of no sequence
+  const int qa = __ldg(p.cu + seq), qe = __ldg(p.cu + seq + 1);
+  if (t < qa || t >= qe) return;  // offsets out of order
+  const int64_t pos = static_cast<int64_t>(__ldg(p.c.lens + seq)) - qe + t;
+  float4 cs[2], sn[2];
+  if (turned) {
+    const int64_t at = pos + (p.offsets != nullptr ? __ldg(p.offsets + seq) : 0);
+    const int64_t row = min(max(at, int64_t(0)), static_cast<int64_t>(p.table_rows) - 1);
+    const float4* cp = reinterpret_cast<const float4*>(p.cos_t + row * (p.rotary / 2) + slot * 8);
+    const float4* sp = reinterpret_cast<const float4*>(p.sin_t + row * (p.rotary / 2) + slot * 8);
+    cs[0] = __ldg(cp);
+    cs[1] = __ldg(cp + 1);
+    sn[0] = __ldg(sp);
+    sn[1] = __ldg(sp + 1);
+  }
+  int64_t dst_kv = -1;  // a position without a slot (negative, past the table, no such page) is not written
+  if (r0 + kAppendRows > p.heads && pos >= 0 && pos < static_cast<int64_t>(p.c.max_pages) * p.c.page_size) {
+    const int idx = static_cast<int>(pos) / p.c.page_size;
+    const int page = __ldg(p.c.table + seq * p.c.table_stride + idx);
+    if (page >= 0 && page < p.c.num_pages)
+      dst_kv = page * p.c.page_stride + (static_cast<int>(pos) - idx * p.c.page_size) * p.c.token_stride;
+  }
+#pragma unroll
+  for (int u = 0; u < 2; ++u) {
+    const int r = r0 + u * 4 + lane / 8;
+    __nv_bfloat16* dst = nullptr;
+    if (r < p.heads) {
+      dst = p.q_out + (static_cast<int64_t>(t) * p.heads + r) * 128;
+    } else if (r < rows && dst_kv >= 0) {
+      const bool is_k = r < p.heads + hk;
+      dst = (is_k ? p.c.k : p.c.v) + dst_kv + (r - p.heads - (is_k ? 0 : hk)) * p.c.head_stride;
+    }
+    if (turned && r < p.heads + hk) {
+      uint32_t* x = reinterpret_cast<uint32_t*>(&a[u]);
+      uint32_t* y = reinterpret_cast<uint32_t*>(&b[u]);
+      const float* c = reinterpret_cast<const float*>(cs);
+      const float* s = reinterpret_cast<const float*>(sn);
+      if (Interleaved) {
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {  // word e of each piece is one pair
+          uint32_t lo = __byte_perm(x[e], y[e], 0x5410), hi = __byte_perm(x[e], y[e], 0x7632);
+          rotate_pairs(lo, hi, make_float2(c[e], c[e + 4]), make_float2(s[e], s[e + 4]));
+          x[e] = __byte_perm(lo, hi, 0x5410);
+          y[e] = __byte_perm(lo, hi, 0x7632);
+        }
+      } else {
+#pragma unroll
+        for (int e = 0; e < 4; ++e)
+          rotate_pairs(x[e], y[e], make_float2(c[2 * e], c[2 * e + 1]), make_float2(s[2 * e], s[2 * e + 1]));
+      }
+    }
+    if (dst != nullptr) {
+      *reinterpret_cast<uint4*>(dst + pa * 8) = a[u];
+      *reinterpret_cast<uint4*>(dst + pb * 8) = b[u];
+    }
+  }
+}
+
+// ------------------------------------------------------------------------------------------------
+// Attention over the pages, 16 rows at a time.
+//
+// O = softmax(scale Q K^T + mask) V and LSE, with the running maximum m and sum l of the softmax kept
+// per row in FP32 (base 2: scores times scale log2 e).
+//
+// For the next tokens of a batch every key and value is read once and 4 sq G FLOP are done per element
+// read, so HBM bounds it: what counts is that all SMs read all the time, whatever the lengths. The
+// rows of all sq new tokens and all G query heads of one K/V head share its keys: row r of a unit is
+// token r / G, head r % G. The work of the launch is one line of 64-key tiles (sequence, K/V head, 16
+// rows, tile), and each block takes an equal stretch of it, so a batch of any lengths is balanced to a
+// tile; a unit that a boundary cuts leaves its pieces in the workspace, and the block that finishes
+// last joins them in the order of their keys (the sum does not depend on who that is).
+//
+// Inside a block the four warps never wait on one another: each takes every fourth 16-key group with
+// its own ring of asynchronous copies, its own m, l and O (16 x 128 in registers, mma.sync m16n8k16),
+// and they are joined once per piece. 16 rows keep the legacy tensor path busy well below its rate at
+// HBM speed: 64 instructions of 4096 multiply-adds for each 8 KiB.
+// ------------------------------------------------------------------------------------------------
+struct PagedParams {
+  PagedCacheView c;
+  const __nv_bfloat16* q;
+  int64_t q_ts, q_hs;
+  const int* cu;       // null: one sequence of all rows
+  __nv_bfloat16* o;    // [total_q, heads, 128]; null: o32
+  float* o32;          // FP32 [total_q, heads, 128], for a result that is joined with another
+  float* lse;          // [heads, total_q] or null
+  const float* add_o;  // another normalised result of the same rows (FP32) with its LSE, joined in; or null
+  const float* add_lse;
+  float* part_o;       // workspace: [2 grid][16][128] and [2 grid][16][2] (m, l)
+  float* part_ml;
+  uint32_t* arrived;   // [grid], zero between launches
+  int heads, group, max_sq, total_q;
+  int causal;
+  float scale_log2;
+};
+
+constexpr int kPagedRows = 16;
+constexpr int kPagedTile = 64;  // keys per tile: one 16-key group per warp
+constexpr int kPagedWarps = 4;
+constexpr int kPagedStages = 3;
+constexpr int kPagedStageBytes = 2 * 16 * 256;  // 16 keys and 16 values
+constexpr int kPagedRing = kPagedStages * kPagedStageBytes;
+constexpr int kPagedPitch = 136;  // floats per row of the joining buffer: 8 rows x 2 floats on 32 banks
+constexpr int kPagedSmem = kPagedWarps * kPagedRing;
+static_assert(kPagedRows * kPagedPitch * 4 <= kPagedRing, "the joining buffer overlays the ring");
+
+__device__ __forceinline__ void cp_async16(uint32_t dst, const void* src, int bytes) {
+  asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(bytes) : "memory");
+}
+__device__ __forceinline__ void cp_async_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
+template <int N>
+__device__ __forceinline__ void cp_async_wait() {
+  asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory");
+}
+__device__ __forceinline__ void ldsm4(uint32_t addr, uint32_t (&r)[4]) {
+  asm volatile("ldmatrix.sync.aligned.m8n8.x4.shared.b16 {%0,%1,%2,%3}, [%4];"
+               : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3])
+               : "r"(addr)
+               : "memory");
+}
+__device__ __forceinline__ void ldsm4_t(uint32_t addr, uint32_t (&r)[4]) {
+  asm volatile("ldmatrix.sync.aligned.m8n8.x4.trans.shared.b16 {%0,%1,%2,%3}, [%4];"
+               : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3])
+               : "r"(addr)
+               : "memory");
+}
+__device__ __forceinline__ void mma16816(float (&d)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
+  asm volatile(
+      "mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+      : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
+      : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+}
+
+// Tiles of one (row block, K/V head) of a sequence; a sequence without keys keeps one, which writes its
+// zero rows.
+__device__ __forceinline__ int paged_tiles(const SeqView& s) {
+  return max((s.len + kPagedTile - 1) / kPagedTile, 1);
+}
+__device__ __forceinline__ int64_t paged_seq_work(const PagedParams& p, const SeqView& s) {
+  if (s.sq == 0) return 0;
+  const int64_t blocks = (static_cast<int64_t>(s.sq) * p.group + kPagedRows - 1) / kPagedRows;
+  return blocks * p.c.kv_heads * paged_tiles(s);
+}
+
+// Row `r` of a unit to its place in the tensors; false past the last row.
+struct RowPlace {
+  int token, head;
+};
+__device__ __forceinline__ bool row_place(const PagedParams& p, const SeqView& s, int h, int64_t r, RowPlace* out) {
+  if (r >= static_cast<int64_t>(s.sq) * p.group) return false;
+  const int i = static_cast<int>(r / p.group);
+  out->token = s.q0 + i;
+  out->head = h * p.group + static_cast<int>(r - static_cast<int64_t>(i) * p.group);
+  return true;
+}
+
+// One finished row: columns 4 lane .. 4 lane + 3 of sum / l, joined with the other result if there is one.
+__device__ __forceinline__ void finish_row(const PagedParams& p, const RowPlace& at, float4 acc, float m, float l,
+                                           int lane) {
+  const int64_t row = static_cast<int64_t>(at.token) * p.heads + at.head;
+  const int64_t lse_at = static_cast<int64_t>(at.head) * p.total_q + at.token;
+  if (p.add_o != nullptr) {
+    const float other = p.add_lse[lse_at] * 1.4426950408889634f;  // base 2; -inf where that result saw no key
+    const float top = fmaxf(m, other);
+    if (top != -INFINITY) {
+      const float w = exp2f(m - top), x = exp2f(other - top);
+      const float4 b = *reinterpret_cast<const float4*>(p.add_o + row * 128 + lane * 4);
+      // where x is 0 the other row is zero
+      acc = make_float4(acc.x * w + b.x * x, acc.y * w + b.y * x, acc.z * w + b.z * x, acc.w * w + b.w * x);
+      l = l * w + x;
+      m = top;
+    }
+  }
+  const float inv = l == 0.f ? 0.f : 1.f / l;  // l is 0 when no key was seen; NaN goes through
+  acc = make_float4(acc.x * inv, acc.y * inv, acc.z * inv, acc.w * inv);
+  if (p.o != nullptr)
+    *reinterpret_cast<uint2*>(p.o + row * 128 + lane * 4) =
+        make_uint2(pack_bf16x2(acc.x, acc.y), pack_bf16x2(acc.z, acc.w));
+  else
+    *reinterpret_cast<float4*>(p.o32 + row * 128 + lane * 4) = acc;
+  if (p.lse != nullptr && lane == 0) p.lse[lse_at] = l == 0.f ? -INFINITY : m * 0.6931471805599453f + logf(l);
+}
+
+__global__ void __launch_bounds__(kPagedWarps * 32, 2) paged_attn_kernel(const __grid_constant__ PagedParams p) {
+  extern __shared__ __align__(1024) uint8_t smem[];
+  __shared__ int64_t scan[kPagedWarps];
+  __shared__ int64_t found_base;
+  __shared__ int found_seq;
+  __shared__ float piece_ml[kPagedWarps][kPagedRows][2];
+  __shared__ uint32_t last_one;
+  const int tid = threadIdx.x, warp = tid / 32, lane = tid % 32;
+
+  // ---- this block's stretch [begin, end) of the line of tiles, and the sequence it begins in ----
+  int64_t total = 0, begin = 0, per = 0;
+  for (int pass = 0; pass < 2; ++pass) {
+    int64_t base = 0;
+    for (int b0 = 0; b0 < p.c.batch; b0 += kPagedWarps * 32) {
+      const int b = b0 + tid;
+      int64_t v = b < p.c.batch ? paged_seq_work(p, seq_view(p.c, p.cu, p.total_q, p.max_sq, b)) : 0;
+      const int64_t mine = v;
+#pragma unroll
+      for (int o = 1; o < 32; o *= 2) {
+        const int64_t up = __shfl_up_sync(0xffffffffu, v, o);
+        if (lane >= o) v += up;
+      }
+      if (lane == 31) scan[warp] = v;
+      __syncthreads();
+      int64_t sum = 0;
+#pragma unroll
+      for (int w = 0; w < kPagedWarps; ++w) {
+        if (w < warp) v += scan[w];
+        sum += scan[w];
+      }
+      if (p.c.batch <= kPagedWarps * 32) {  // one step sees the whole batch: no second pass
+        total = sum;
+        per = (total + gridDim.x - 1) / gridDim.x;
+        begin = blockIdx.x * per;
+        pass = 1;
+      }
+      if (pass == 1 && base + v - mine <= begin && begin < base + v) {
+        found_seq = b;
+        found_base = base + v - mine;
+      }
+      base += sum;
+      __syncthreads();
+    }
+    if (pass == 0) {
+      total = base;
+      per = (total + gridDim.x - 1) / gridDim.x;
+      begin = blockIdx.x * per;
+    }
+  }
+  const int64_t end = min(total, begin + per);
+  if (begin >= end) return;
+  int b = found_seq;
+  int64_t base = found_base;
+
+  const uint32_t ring = smem_addr(smem) + warp * kPagedRing;
+  float* join = reinterpret_cast<float*>(smem + warp * kPagedRing);
+
+  for (int64_t pos = begin; pos < end;) {
+    const SeqView s = seq_view(p.c, p.cu, p.total_q, p.max_sq, b);
+    const int64_t work = paged_seq_work(p, s);
+    if (pos >= base + work) {  // this sequence is done
+      base += work;
+      ++b;
+      continue;
+    }
+    const int n = paged_tiles(s);
+    const int blocks = static_cast<int>((static_cast<int64_t>(s.sq) * p.group + kPagedRows - 1) / kPagedRows);
+    const int64_t unit = (pos - base) / n;
+    const int tile0 = static_cast<int>(pos - base - unit * n);
+    const int cnt = static_cast<int>(min(static_cast<int64_t>(n - tile0), end - pos));
+    const int h = static_cast<int>(unit / blocks);
+    const int64_t r0 = (unit - static_cast<int64_t>(h) * blocks) * kPagedRows;
+
+    // last visible key of this thread's rows (g and g + 8), and of the whole row block
+    const int g = lane / 4, t4 = lane % 4;
+    const int64_t rows = static_cast<int64_t>(s.sq) * p.group;
+    const int past = s.len - s.sq;
+    int lim[2];
+#pragma unroll
+    for (int u = 0; u < 2; ++u) {
+      const int64_t r = min(r0 + g + 8 * u, rows - 1);
+      lim[u] = p.causal ? past + static_cast<int>(r / p.group) : s.len - 1;
+    }
+    const int lim_max =
+        p.causal ? past + static_cast<int>(min(r0 + kPagedRows - 1, rows - 1) / p.group) : s.len - 1;
+    const int lim_min = p.causal ? past + static_cast<int>(r0 / p.group) : s.len - 1;
+    const int key_begin = tile0 * kPagedTile;
+    const int64_t key_stop = static_cast<int64_t>(tile0 + cnt) * kPagedTile;
+    const int key_end = static_cast<int>(min(key_stop, static_cast<int64_t>(min(s.len, lim_max + 1))));
+    const int groups = max(key_end - key_begin + 15, 0) / 16;
+    const int steps = (groups - warp + kPagedWarps - 1) / kPagedWarps;  // this warp's 16-key groups (<= 0: none)
+
+    // ring: lane copies piece lane % 16 of rows lane / 16 + 2 j
+    const int64_t head_off = h * p.c.head_stride;
+    const int* table = p.c.table + b * p.c.table_stride;
+    const int cl = lane % 16, rl = lane / 16;
+    auto key_of = [&](int i) { return key_begin + (warp + kPagedWarps * i) * 16; };
+    auto page_of = [&](int i) { return i < steps ? __ldg(table + key_of(i) / p.c.page_size) : 0; };
+    auto issue = [&](int i, int page) {
+      if (i < steps) {
+        const int key = key_of(i);
+        page = min(max(page, 0), p.c.num_pages - 1);
+        const int64_t off = page * p.c.page_stride + (key % p.c.page_size + rl) * p.c.token_stride + head_off + cl * 8;
+        const __nv_bfloat16* ks = p.c.k + off;
+        const __nv_bfloat16* vs = p.c.v + off;
+        const uint32_t dst = ring + (i % kPagedStages) * kPagedStageBytes + rl * 256;
+#pragma unroll
+        for (int j = 0; j < 8; ++j) {
+          const int row = rl + 2 * j;
+          const int bytes = key + row < s.len ? 16 : 0;  // slots past the end may hold anything: zeros instead
+          const uint32_t d = dst + j * 512 + ((cl ^ (row & 7)) * 16);
+          cp_async16(d, ks + 2 * j * p.c.token_stride, bytes);
+          cp_async16(d + 4096, vs + 2 * j * p.c.token_stride, bytes);
+        }
+      }
+      cp_async_commit();
+    };
+    int page_next = page_of(0);
+#pragma unroll
+    for (int i = 0; i < kPagedStages - 1; ++i) {
+      const int page = page_next;
+      page_next = page_of(i + 1);
+      issue(i, page);
+    }
+    uint32_t qf[8][4];
+#pragma unroll
+    for (int u = 0; u < 2; ++u) {
+      RowPlace at;
+      const bool live = row_place(p, s, h, r0 + g + 8 * u, &at);
+      const __nv_bfloat16* src = live ? p.q + at.token * p.q_ts + at.head * p.q_hs + t4 * 2 : nullptr;
+#pragma unroll
+      for (int k = 0; k < 8; ++k) {
+        qf[k][u] = live ? __ldg(reinterpret_cast<const uint32_t*>(src + k * 16)) : 0u;
+        qf[k][u + 2] = live ? __ldg(reinterpret_cast<const uint32_t*>(src + k * 16 + 8)) : 0u;
+      }
+    }
+
+    float o[16][4];
+#pragma unroll
+    for (int j = 0; j < 16; ++j) o[j][0] = o[j][1] = o[j][2] = o[j][3] = 0.f;
+    float m[2] = {-INFINITY, -INFINITY}, l[2] = {0.f, 0.f};
+    const int mi = lane / 8, mr = lane % 8;
+    for (int i = 0; i < steps; ++i) {
+      cp_async_wait<kPagedStages - 2>();
+      __syncwarp();  // group i has arrived, and every lane is done with group i - 1
+      const int page = page_next;
+      page_next = page_of(i + kPagedStages);
+      issue(i + kPagedStages - 1, page);
+      const uint32_t st = ring + (i % kPagedStages) * kPagedStageBytes;
+      float sc[2][4] = {};
+#pragma unroll
+      for (int k = 0; k < 8; ++k) {
+        uint32_t kb[4];
+        ldsm4(st + ((mi / 2) * 8 + mr) * 256 + (((2 * k + (mi & 1)) ^ mr) * 16), kb);
+        mma16816(sc[0], qf[k], kb[0], kb[1]);
+        mma16816(sc[1], qf[k], kb[2], kb[3]);
+      }
+      const int key = key_of(i);
+      if (key + 15 > lim_min) {
+#pragma unroll
+        for (int e = 0; e < 8; ++e) {
+          const int col = key + (e / 4) * 8 + t4 * 2 + (e & 1);
+          if (col > lim[(e / 2) & 1]) sc[e / 4][e % 4] = -INFINITY;
+        }
+      }
+      bool grow = false;
+      float cand[2];
+#pragma unroll
+      for (int u = 0; u < 2; ++u) {
+        float mx = fmaxf(fmaxf(sc[0][2 * u], sc[0][2 * u + 1]), fmaxf(sc[1][2 * u], sc[1][2 * u + 1]));
+        mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 1));
+        mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 2));
+        cand[u] = fmaxf(m[u], mx * p.scale_log2);
+        grow |= cand[u] > m[u] + 8.f;  // the sums are rescaled only when a maximum grows by 2^8
+      }
+      if (__any_sync(0xffffffffu, grow)) {
+#pragma unroll
+        for (int u = 0; u < 2; ++u) {
+          const float a = cand[u] == -INFINITY ? 1.f : ex2_mufu(m[u] - cand[u]);
+          m[u] = cand[u];
+          l[u] *= a;
+#pragma unroll
+          for (int j = 0; j < 16; ++j) {
+            o[j][2 * u] *= a;
+            o[j][2 * u + 1] *= a;
+          }
+        }
+      }
+      uint32_t pf[4];
+#pragma unroll
+      for (int u = 0; u < 2; ++u) {
+        const float mb = m[u] == -INFINITY ? 0.f : m[u];
+        const float p0 = ex2_mufu(fmaf(sc[0][2 * u], p.scale_log2, -mb));
+        const float p1 = ex2_mufu(fmaf(sc[0][2 * u + 1], p.scale_log2, -mb));
+        const float p2 = ex2_mufu(fmaf(sc[1][2 * u], p.scale_log2, -mb));
+        const float p3 = ex2_mufu(fmaf(sc[1][2 * u + 1], p.scale_log2, -mb));
+        l[u] += (p0 + p1) + (p2 + p3);
+        pf[u] = pack_bf16x2(p0, p1);  // P in BF16 for the second product; l sums the unrounded values
+        pf[u + 2] = pack_bf16x2(p2, p3);
+      }
+#pragma unroll
+      for (int j = 0; j < 8; ++j) {
+        uint32_t vb[4];
+        ldsm4_t(st + 4096 + ((mi & 1) * 8 + mr) * 256 + (((2 * j + mi / 2) ^ mr) * 16), vb);
+        mma16816(o[2 * j], pf, vb[0], vb[1]);
+        mma16816(o[2 * j + 1], pf, vb[2], vb[3]);
+      }
+    }
+
+    // ---- join the four warps ----
+    cp_async_wait<0>();
+    __syncwarp();
+#pragma unroll
+    for (int u = 0; u < 2; ++u) {
+      l[u] += __shfl_xor_sync(0xffffffffu, l[u], 1);
+      l[u] += __shfl_xor_sync(0xffffffffu, l[u], 2);
+      if (t4 == 0) {
+        piece_ml[warp][g + 8 * u][0] = m[u];
+        piece_ml[warp][g + 8 * u][1] = l[u];
+      }
+#pragma unroll
+      for (int j = 0; j < 16; ++j)
+        *reinterpret_cast<float2*>(join + (g + 8 * u) * kPagedPitch + j * 8 + t4 * 2) =
+            make_float2(o[j][2 * u], o[j][2 * u + 1]);
+    }
+    __syncthreads();
+    const bool whole = cnt == n;
+    const int slot = 2 * blockIdx.x + (tile0 == 0 ? 1 : 0);  // a piece that opens its unit, or one that carries on
+    for (int r = warp; r < kPagedRows && r0 + r < rows; r += kPagedWarps) {
+      float top = piece_ml[0][r][0];
+#pragma unroll
+      for (int w = 1; w < kPagedWarps; ++w) top = fmaxf(top, piece_ml[w][r][0]);
+      float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
+      float sum = 0.f;
+#pragma unroll
+      for (int w = 0; w < kPagedWarps; ++w) {
+        const float mw = piece_ml[w][r][0];
+        const float a = mw == -INFINITY ? 0.f : exp2f(mw - top);
+        const float4 v =
+            *reinterpret_cast<const float4*>(reinterpret_cast<float*>(smem + w * kPagedRing) + r * kPagedPitch + lane * 4);
+        acc = make_float4(acc.x + a * v.x, acc.y + a * v.y, acc.z + a * v.z, acc.w + a * v.w);
+        sum += a * piece_ml[w][r][1];
+      }
+      if (whole) {
+        RowPlace at;
+        row_place(p, s, h, r0 + r, &at);
+        finish_row(p, at, acc, top, sum, lane);
+      } else {
+        *reinterpret_cast<float4*>(p.part_o + (static_cast<int64_t>(slot) * kPagedRows + r) * 128 + lane * 4) = acc;
+        if (lane == 0)
+          *reinterpret_cast<float2*>(p.part_ml + (static_cast<int64_t>(slot) * kPagedRows + r) * 2) =
+              make_float2(top, sum);
+      }
+    }
+    if (!whole) {
+      // the blocks of this unit: from the one that holds its first tile to the one that holds its last
+      const int64_t first_pos = pos - tile0;
+      const int c0 = static_cast<int>(first_pos / per), c1 = static_cast<int>((first_pos + n - 1) / per);
+      __threadfence();
+      __syncthreads();
+      if (tid == 0) {
+        const uint32_t before = atomicAdd(p.arrived + c0, 1u);
+        last_one = before == static_cast<uint32_t>(c1 - c0);
+        if (last_one) p.arrived[c0] = 0u;  // ready for the next launch
+      }
+      __syncthreads();
+      if (last_one) {
+        __threadfence();
+        for (int r = warp; r < kPagedRows && r0 + r < rows; r += kPagedWarps) {
+          auto slot_row = [&](int c) { return static_cast<int64_t>(2 * c + (c == c0 ? 1 : 0)) * kPagedRows + r; };
+          float top = -INFINITY;
+          for (int c = c0 + lane; c <= c1; c += 32) top = fmaxf(top, __ldcg(p.part_ml + slot_row(c) * 2));
+#pragma unroll
+          for (int x = 16; x > 0; x /= 2) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, x));
+          float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
+          float sum = 0.f;
+          for (int c = c0; c <= c1; c += 8) {
+            float4 v[8];
+            float2 ml[8];
+#pragma unroll
+            for (int x = 0; x < 8; ++x) {
+              if (c + x <= c1) {
+                v[x] = __ldcg(reinterpret_cast<const float4*>(p.part_o + slot_row(c + x) * 128 + lane * 4));
+                ml[x] = __ldcg(reinterpret_cast<const float2*>(p.part_ml + slot_row(c + x) * 2));
+              }
+            }
+#pragma unroll
+            for (int x = 0; x < 8; ++x) {
+              if (c + x <= c1 && ml[x].x != -INFINITY) {
+                const float a = exp2f(ml[x].x - top);
+                acc = make_float4(acc.x + a * v[x].x, acc.y + a * v[x].y, acc.z + a * v[x].z, acc.w + a * v[x].w);
+                sum += a * ml[x].y;
+              }
+            }
+          }
+          RowPlace at;
+          row_place(p, s, h, r0 + r, &at);
+          finish_row(p, at, acc, top, sum, lane);
+        }
+      }
+    }
+    pos += cnt;
+    __syncthreads();  // the joining buffer is the ring of the next piece
+  }
+}
+
+}  // namespace fav4

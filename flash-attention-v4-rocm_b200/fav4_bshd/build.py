@@ -2,8 +2,8 @@
 
     python -m fav4_bshd.build [--force]
 
-Compiles csrc/fav4_bshd.cu -> build/libfav4_bshd.so (the C ABI of
-include/fav4_bshd.h) and csrc/probe.cu -> build/libfav4_probe.so (test probes)
+Compiles csrc/fav4_bshd.cu and csrc/paged.cu -> build/libfav4_bshd.so (the C
+ABI of include/fav4_bshd.h) and csrc/probe.cu -> build/libfav4_probe.so (test probes)
 with nvcc for sm_100a, statically linked against the CUDA runtime. The ptxas
 resource report (registers, spills, shared memory) of each build is written
 next to the library as build/<lib>.ptxas.txt.
@@ -26,7 +26,7 @@ ARCH_FLAGS = ["-gencode", "arch=compute_100a,code=sm_100a"]
 COMMON = ["-O3", "-lineinfo", "-std=c++17", "-Xcompiler", "-fPIC", "-shared", "-Xptxas", "-v",
           f"-I{INCLUDE}", f"-I{CSRC}"]
 TARGETS = {
-    "libfav4_bshd.so": ["fav4_bshd.cu"],
+    "libfav4_bshd.so": ["fav4_bshd.cu", "paged.cu"],
     "libfav4_probe.so": ["probe.cu"],
 }
 

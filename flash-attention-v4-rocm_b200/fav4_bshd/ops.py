@@ -28,6 +28,11 @@ composes with both. Gradients of O with respect to q, k, v come from
 attention: dK and dV of a K/V head sum over its query heads); they need the
 LSE, so call the op with ``return_lse=True`` (``attention()`` does). A gradient
 through the LSE output is not implemented and raises.
+
+``torch.ops.fav4.paged_append``, ``paged_forward`` and ``shared_prefix_forward`` are
+the calls of fav4_bshd.paged (serving from a paged key/value cache): packed
+queries ``[T, H, 128]``, caches ``[pages, page_size, H_kv, 128]``, device int32
+tables and lengths. paged_append mutates the caches; none of them has a gradient.
 """
 from __future__ import annotations
 
@@ -35,7 +40,7 @@ import math
 
 import torch
 
-from . import HEAD_DIM, Runner
+from . import HEAD_DIM, Runner, paged
 
 _RUNNER: Runner | None = None
 
@@ -188,3 +193,93 @@ def attention(q, k, v, causal: bool = False, config: int = 0, scale: float | Non
     is always computed so that the backward pass can use it)."""
     o, lse = torch.ops.fav4.bshd_forward(q, k, v, causal, config, -1.0 if scale is None else scale, True)
     return (o, lse) if return_lse else o
+
+
+def _check_paged(q, k_cache, v_cache, page_table, seq_lens, cu_q):
+    torch._check(q.dim() == 3 and q.shape[-1] == HEAD_DIM, lambda: f"q must be [T, H, {HEAD_DIM}], got {q.shape}")
+    torch._check(k_cache.dim() == 4 and k_cache.shape == v_cache.shape and k_cache.shape[3] == HEAD_DIM
+                 and k_cache.shape[1] % 16 == 0,
+                 lambda: f"caches must be [pages, page_size, H_kv, {HEAD_DIM}] with page_size a multiple of 16, got "
+                         f"{k_cache.shape} and {v_cache.shape}")
+    torch._check(all(x.dtype == torch.bfloat16 for x in (q, k_cache, v_cache)), lambda: "q and the caches must be bfloat16")
+    torch._check(k_cache.stride() == v_cache.stride() and k_cache.stride(3) == 1 and q.stride(2) == 1,
+                 lambda: "the caches must have one layout, and every row contiguous elements")
+    torch._check(all(x.dtype == torch.int32 for x in (page_table, seq_lens, cu_q)),
+                 lambda: "page_table, seq_lens and cu_q must be int32")
+    torch._check(page_table.dim() == 2 and seq_lens.shape == page_table.shape[:1]
+                 and cu_q.dim() == 1 and cu_q.shape[0] == page_table.shape[0] + 1,
+                 lambda: "page_table must be [B, max_pages], seq_lens [B] and cu_q [B + 1]")
+
+
+@torch.library.custom_op("fav4::paged_append", mutates_args=("k_cache", "v_cache"), device_types="cuda")
+def paged_append(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor,
+                 page_table: torch.Tensor, seq_lens: torch.Tensor, cu_q: torch.Tensor, cos: torch.Tensor | None,
+                 sin: torch.Tensor | None, interleaved: bool, offsets: torch.Tensor | None) -> torch.Tensor:
+    """fav4_bshd.paged.append: the rotated queries; k_cache and v_cache are written."""
+    _check_append(q, k, v, k_cache, v_cache, page_table, seq_lens, cu_q, cos, sin)
+    return paged.append(q, k, v, k_cache, v_cache, page_table, seq_lens.contiguous(), cu_q.contiguous(), cos, sin,
+                        interleaved=interleaved, offsets=offsets)
+
+
+def _check_append(q, k, v, k_cache, v_cache, page_table, seq_lens, cu_q, cos, sin):
+    _check_paged(q, k_cache, v_cache, page_table, seq_lens, cu_q)
+    torch._check(k.shape == v.shape == (q.shape[0], k_cache.shape[2], HEAD_DIM),
+                 lambda: f"k and v must be [T, H_kv, {HEAD_DIM}], got {k.shape} and {v.shape}")
+    torch._check(k.dtype == torch.bfloat16 and v.dtype == torch.bfloat16, lambda: "k and v must be bfloat16")
+    torch._check((cos is None) == (sin is None), lambda: "cos and sin come together")
+    if cos is not None:
+        torch._check(cos.dim() == 2 and cos.shape == sin.shape and cos.shape[1] % 8 == 0 and cos.shape[1] <= 64
+                     and cos.dtype == torch.float32 and sin.dtype == torch.float32,
+                     lambda: "cos and sin must be FP32 [positions, rotary / 2] with rotary a multiple of 16 up to 128")
+
+
+@paged_append.register_fake
+def _(q, k, v, k_cache, v_cache, page_table, seq_lens, cu_q, cos, sin, interleaved, offsets):
+    _check_append(q, k, v, k_cache, v_cache, page_table, seq_lens, cu_q, cos, sin)
+    return torch.empty_like(q, memory_format=torch.contiguous_format)
+
+
+@torch.library.custom_op("fav4::paged_forward", mutates_args=(), device_types="cuda")
+def paged_forward(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor, page_table: torch.Tensor,
+                  seq_lens: torch.Tensor, cu_q: torch.Tensor, max_sq: int, causal: bool,
+                  scale: float) -> tuple[torch.Tensor, torch.Tensor]:
+    """fav4_bshd.paged.attention: O [T, H, 128] and LSE (FP32 [H, T]); a non-positive scale is 1/sqrt(128)."""
+    _check_paged(q, k_cache, v_cache, page_table, seq_lens, cu_q)
+    return paged.attention(q, k_cache, v_cache, page_table, seq_lens.contiguous(), cu_q.contiguous(), max_sq,
+                           causal=causal, scale=None if scale <= 0 else scale, return_lse=True)
+
+
+def _fake_attend(q):
+    return torch.empty_like(q, memory_format=torch.contiguous_format), q.new_empty((q.shape[1], q.shape[0]),
+                                                                                   dtype=torch.float32)
+
+
+@paged_forward.register_fake
+def _(q, k_cache, v_cache, page_table, seq_lens, cu_q, max_sq, causal, scale):
+    _check_paged(q, k_cache, v_cache, page_table, seq_lens, cu_q)
+    return _fake_attend(q)
+
+
+@torch.library.custom_op("fav4::shared_prefix_forward", mutates_args=(), device_types="cuda")
+def shared_prefix_forward(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor, prefix_pages: torch.Tensor,
+                          prefix_len: torch.Tensor, page_table: torch.Tensor, seq_lens: torch.Tensor,
+                          cu_q: torch.Tensor, max_sq: int, causal: bool,
+                          scale: float) -> tuple[torch.Tensor, torch.Tensor]:
+    """fav4_bshd.paged.shared_prefix_attention: O [T, H, 128] and LSE (FP32 [H, T])."""
+    _check_prefix(q, k_cache, v_cache, prefix_pages, prefix_len, page_table, seq_lens, cu_q)
+    return paged.shared_prefix_attention(q, k_cache, v_cache, prefix_pages, prefix_len, page_table,
+                                         seq_lens.contiguous(), cu_q.contiguous(), max_sq, causal=causal,
+                                         scale=None if scale <= 0 else scale, return_lse=True)
+
+
+def _check_prefix(q, k_cache, v_cache, prefix_pages, prefix_len, page_table, seq_lens, cu_q):
+    _check_paged(q, k_cache, v_cache, page_table, seq_lens, cu_q)
+    torch._check(prefix_pages.dim() == 1 and prefix_pages.shape[0] >= 1 and prefix_len.numel() == 1
+                 and prefix_pages.dtype == torch.int32 and prefix_len.dtype == torch.int32,
+                 lambda: "prefix_pages must be int32 [n], n >= 1, and prefix_len int32 [1]")
+
+
+@shared_prefix_forward.register_fake
+def _(q, k_cache, v_cache, prefix_pages, prefix_len, page_table, seq_lens, cu_q, max_sq, causal, scale):
+    _check_prefix(q, k_cache, v_cache, prefix_pages, prefix_len, page_table, seq_lens, cu_q)
+    return _fake_attend(q)

@@ -288,6 +288,104 @@ size_t fav4_bshd_host_workspace_bytes(const Fav4Args* args, const Fav4HostOut* o
 int fav4_bshd_forward_host(const Fav4Args* args, const Fav4HostOut* outs, int n_outs, int chunks, void* workspace,
                            size_t workspace_bytes, cudaStream_t stream);
 
+/* Paged key/value cache (no reference counterpart: the reference attends one
+ * contiguous K/V). k and v are BF16 arrays of num_pages pages of page_size keys
+ * (a multiple of 16); element (page, slot, head, d) of either is at
+ * page * page_stride + slot * token_stride + head * head_stride + d, strides in
+ * elements and multiples of 8, so [page][slot][head][128] and
+ * [page][head][slot][128] layouts both work. Key s of sequence b is in slot
+ * s % page_size of page page_table[b * table_stride + s / page_size]; the table
+ * has max_pages entries per sequence, of which the first
+ * ceil(seq_lens[b] / page_size) are used. page_table and seq_lens are device
+ * int32; seq_lens[b] counts every key, this call's new ones included. Lengths
+ * are clamped to [0, max_pages * page_size] and page numbers to the cache:
+ * malformed ones give wrong rows, never an access outside the arrays. Slots past
+ * a sequence's end may hold anything, NaN included. */
+struct Fav4PagedCache {
+  void *k, *v;
+  const int* page_table;
+  const int* seq_lens;
+  long long page_stride, token_stride, head_stride, table_stride;
+  int batch, kv_heads, num_pages, page_size, max_pages;
+};
+typedef struct Fav4PagedCache Fav4PagedCache;
+
+/* Appends new keys and values to the cache and rotates queries and keys on the
+ * way (rotary position embedding). q [total_q, heads, 128], k and v [total_q,
+ * kv_heads, 128]: BF16 with the given strides (elements, multiples of 8; e.g.
+ * slices of one fused projection). Sequence b's new rows are [cu_seqlens_q[b],
+ * cu_seqlens_q[b+1]) (device int32, batch + 1 of them) and its row i gets
+ * position seq_lens[b] - (cu_seqlens_q[b+1] - cu_seqlens_q[b]) + i: its slot in
+ * the cache, and (plus offsets[b] when offsets is not NULL, device int32
+ * [batch]) its row of cos_table / sin_table, FP32 [table_rows, rotary_dim / 2],
+ * clamped to the table. The first rotary_dim elements (a multiple of 16, at most
+ * 128, 0 for none) of q's and k's heads are rotated by (x cos - y sin, y cos + x
+ * sin): pairs are (i, i + rotary_dim / 2), or (2i, 2i + 1) when interleaved.
+ * q_out: BF16 [total_q, heads, 128], contiguous; it may be q's own memory when q
+ * is contiguous. A row whose position is negative or whose page number is outside
+ * the cache writes no key; rows of no sequence write nothing. Pages that two
+ * sequences share must not be appended to. Returns 0, cudaErrorInvalidValue or
+ * the launch status. */
+struct Fav4PagedAppendArgs {
+  Fav4PagedCache cache;
+  const void *q, *k, *v;
+  void* q_out;
+  const int* cu_seqlens_q;
+  const float *cos_table, *sin_table;
+  const int* offsets;
+  long long q_token_stride, q_head_stride, k_token_stride, k_head_stride, v_token_stride, v_head_stride;
+  int heads, total_q, rotary_dim, interleaved, table_rows;
+};
+typedef struct Fav4PagedAppendArgs Fav4PagedAppendArgs;
+
+int fav4_bshd_paged_append(const Fav4PagedAppendArgs* args, cudaStream_t stream);
+
+/* Attention over the cache's pages, for next tokens and for chunks of prompts.
+ * q: BF16 [total_q, heads, 128] with the given strides; sequence b's rows are
+ * [cu_seqlens_q[b], cu_seqlens_q[b+1]), at most max_sq of them (rows past max_sq
+ * are not computed). Query head h attends K/V head h / (heads / kv_heads). With
+ * causal = 1 the rows are a sequence's newest keys: row i of sq sees keys [0,
+ * seq_lens[b] - sq + i] (bottom-right, unlike the top-left mask of
+ * fav4_bshd_forward; the same where sq = sk). With causal = 0 every row sees
+ * every key. o: BF16 [total_q, heads, 128], contiguous; lse: optional FP32
+ * [heads, total_q], natural log. A row that sees no key gets O = 0 and LSE =
+ * -inf.
+ *
+ * Shared prefix: prefix_len (device int32 [1]) keys at prefix_pages (device int32
+ * [max_prefix_pages], pages of the same cache) stand before every sequence's own
+ * keys and are seen by every row; seq_lens and page_table then count and name the
+ * own keys only. The prefix is read once for the whole batch instead of once per
+ * sequence. fav4_bshd_forward_paged wants prefix_pages NULL,
+ * fav4_bshd_forward_shared_prefix wants both pointers.
+ *
+ * workspace: device memory, 256-byte aligned, of
+ * fav4_bshd_paged_workspace_bytes(args) bytes, the first 4096 of them (counters)
+ * zero before its first use; every call leaves them zero, so calls of any
+ * arguments may follow one another. Calls sharing a workspace must not overlap. The
+ * result does not depend on scheduling: the same call gives the same bits.
+ * Return 0, cudaErrorInvalidValue or the launch status. */
+struct Fav4PagedArgs {
+  Fav4PagedCache cache;
+  const void* q;
+  void* o;
+  float* lse;
+  const int* cu_seqlens_q;
+  const int* prefix_pages;
+  const int* prefix_len;
+  long long q_token_stride, q_head_stride;
+  int heads, max_sq, total_q, max_prefix_pages;
+  float scale;
+};
+typedef struct Fav4PagedArgs Fav4PagedArgs;
+
+/* Workspace of the two calls below (0 on invalid arguments). It depends on heads,
+ * max_sq, total_q and whether there is a prefix, not on the lengths. */
+size_t fav4_bshd_paged_workspace_bytes(const Fav4PagedArgs* args);
+int fav4_bshd_forward_paged(const Fav4PagedArgs* args, int causal, void* workspace, size_t workspace_bytes,
+                            cudaStream_t stream);
+int fav4_bshd_forward_shared_prefix(const Fav4PagedArgs* args, int causal, void* workspace, size_t workspace_bytes,
+                                    cudaStream_t stream);
+
 /* Failure detection (no reference counterpart): every pipeline wait inside the
  * kernels is bounded in time (default 2000 ms, environment variable
  * FAV4_WAIT_LIMIT_MS). A wait that runs out makes the kernel stop cleanly and
