@@ -21,6 +21,7 @@
 #include "attn_bwd_sm100.cuh"
 #include "attn_bwd_fused_sm100.cuh"
 #include "combine.cuh"
+#include "host_status.h"
 #include "tensor_map.h"
 #include "fav4_bshd.h"
 
@@ -68,6 +69,17 @@ bool device_info(int dev, DeviceInfo* out) {
   *out = cache[dev];
   return true;
 }
+
+}  // namespace
+
+uint32_t* pipeline_status_word() {
+  int dev = 0;
+  DeviceInfo info;
+  return cudaGetDevice(&dev) == cudaSuccess && device_info(dev, &info) ? info.status : nullptr;
+}
+uint64_t pipeline_wait_limit_ns() { return wait_limit_ns(); }
+
+namespace {
 
 // The reference's argument checks (src/bshd.hip:27-34).
 bool args_valid(const Fav4Args* a, int causal, int config) {

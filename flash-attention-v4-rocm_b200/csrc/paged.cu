@@ -8,13 +8,16 @@
 #include <mutex>
 
 #include "fav4_bshd.h"
+#include "host_status.h"
 #include "paged.cuh"
+#include "paged_tile_sm100.cuh"
+#include "tensor_map.h"
 
 namespace fav4 {
 namespace {
 
 constexpr int kMaxDevices = 64;
-constexpr int kMaxSms = 256;         // bound on the SMs that the workspace is laid out for
+constexpr int kMaxSms = 160;         // bound on the SMs that the workspace is laid out for (a B200 has 148)
 constexpr int kPagedPerSm = 2;       // blocks of paged_attn_kernel per SM
 constexpr int kMaxGrid = kMaxSms * kPagedPerSm;
 
@@ -37,6 +40,10 @@ int sm_count(int* sms) {
     e = cudaDeviceGetAttribute(&n, cudaDevAttrMultiProcessorCount, dev);
     if (e != cudaSuccess) return e;
     e = cudaFuncSetAttribute(paged_attn_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, kPagedSmem);
+    if (e != cudaSuccess) return e;
+    e = cudaFuncSetAttribute(paged_tile_kernel<1>, cudaFuncAttributeMaxDynamicSharedMemorySize, PagedTileLayout<1>::kAlloc);
+    if (e != cudaSuccess) return e;
+    e = cudaFuncSetAttribute(paged_tile_kernel<2>, cudaFuncAttributeMaxDynamicSharedMemorySize, PagedTileLayout<2>::kAlloc);
     if (e != cudaSuccess) return e;
     count[dev] = n < kMaxSms ? n : kMaxSms;
   }
@@ -100,25 +107,94 @@ bool paged_valid(const Fav4PagedArgs* a) {
          stride_ok(a->q_token_stride) && stride_ok(a->q_head_stride);
 }
 
-// Workspace: counters first (their place never changes, so that any call may follow any other), then
-// the pieces of cut units, then the prefix's result.
+// Rows of one sequence's new tokens (of all rows, against a prefix) that share a K/V head, and the Q tiles
+// per block that they get: 0 for paged_attn_kernel's 16 rows.
+int q_tiles(long long tokens, int group) {
+  const long long rows = tokens * group;
+  return rows <= kPagedRows || group > kBlockM ? 0 : rows <= kBlockM ? 1 : 2;
+}
+
+// Workspace: counters first (their place never changes, so that any call may follow any other), then the
+// pieces of cut units (of whichever kernel needs more), then the first of a prefixed call's two results.
 struct PagedSpace {
-  size_t part_o, part_ml, prefix_o, prefix_lse, total;
-  static constexpr size_t kCounters = 2 * kMaxGrid * sizeof(uint32_t);  // own keys, prefix
+  size_t part_o, part_ml, tile_o, tile_ml, cut, first_o, first_lse, total;
+  static constexpr size_t kCounters = 4096;
 };
+static_assert(2 * kMaxGrid * sizeof(uint32_t) <= PagedSpace::kCounters, "two calls' counters");
+static_assert(kMaxSms <= 256, "paged_join_kernel reads one cut unit per thread");
 PagedSpace paged_space(const Fav4PagedArgs& a) {
+  const int group = a.heads / a.cache.kv_heads;
+  int tiles = q_tiles(a.max_sq, group);
+  if (a.prefix_pages && q_tiles(a.total_q, group) > tiles) tiles = q_tiles(a.total_q, group);
   PagedSpace s;
   s.part_o = PagedSpace::kCounters;
   s.part_ml = s.part_o + size_t(2) * kMaxGrid * kPagedRows * 128 * sizeof(float);
-  s.prefix_o = s.part_ml + size_t(2) * kMaxGrid * kPagedRows * 2 * sizeof(float);
-  s.prefix_lse = s.prefix_o;
-  s.total = s.prefix_o;
+  s.tile_o = s.part_ml + size_t(2) * kMaxGrid * kPagedRows * 2 * sizeof(float);
+  s.tile_ml = s.tile_o + size_t(2) * kMaxSms * tiles * kBlockM * 128 * sizeof(float);
+  s.cut = s.tile_ml + size_t(2) * kMaxSms * tiles * kBlockM * 2 * sizeof(float);
+  s.first_o = s.cut + round256(kMaxSms * sizeof(int4));
+  s.first_lse = s.total = s.first_o;
   if (a.prefix_pages) {
     const size_t rows = static_cast<size_t>(a.total_q) * a.heads;
-    s.prefix_lse = s.prefix_o + round256(rows * 128 * sizeof(float));
-    s.total = s.prefix_lse + round256(rows * sizeof(float));
+    s.first_lse = s.first_o + round256(rows * 128 * sizeof(float));
+    s.total = s.first_lse + round256(rows * sizeof(float));
   }
   return s;
+}
+
+bool encode_cache(CUtensorMap* map, const __nv_bfloat16* base, const PagedCacheView& c, int box_rows) {
+  const cuuint64_t dims[4] = {128, static_cast<cuuint64_t>(c.kv_heads), static_cast<cuuint64_t>(c.page_size),
+                              static_cast<cuuint64_t>(c.num_pages)};
+  const long long strides[4] = {1, c.head_stride, c.token_stride, c.page_stride};
+  const cuuint32_t box[4] = {64, 1, static_cast<cuuint32_t>(box_rows), 1};
+  return encode_rows(map, base, 4, dims, strides, box);
+}
+
+template <int QTiles>
+int launch_tiles(const PagedParams& p, const PagedSpace& sp, uint8_t* ws, int sms, cudaStream_t stream) {
+  PagedTileParams t;
+  t.p = p;
+  t.p.part_o = reinterpret_cast<float*>(ws + sp.tile_o);
+  t.p.part_ml = reinterpret_cast<float*>(ws + sp.tile_ml);
+  t.cut = reinterpret_cast<int4*>(ws + sp.cut);
+  t.tile_tokens = kBlockM / p.group;
+  t.box_rows = 16;  // the largest power of two up to 128 that divides the page size
+  while (t.box_rows < kTileKeys && p.c.page_size % (2 * t.box_rows) == 0) t.box_rows *= 2;
+  t.status = pipeline_status_word();
+  t.wait_limit_ns = pipeline_wait_limit_ns();
+  if (!t.status) return cudaErrorInvalidDevice;
+  CUtensorMap tq, tk, tv;
+  const cuuint64_t dims[3] = {128, static_cast<cuuint64_t>(p.heads), static_cast<cuuint64_t>(p.total_q)};
+  const long long strides[3] = {1, p.q_hs, p.q_ts};
+  const cuuint32_t box[3] = {64, static_cast<cuuint32_t>(p.group), static_cast<cuuint32_t>(t.tile_tokens)};
+  if (!encode_rows(&tq, p.q, 3, dims, strides, box) || !encode_cache(&tk, p.c.k, p.c, t.box_rows) ||
+      !encode_cache(&tv, p.c.v, p.c, t.box_rows))
+    return cudaErrorInvalidValue;
+  paged_tile_kernel<QTiles><<<sms, 384, PagedTileLayout<QTiles>::kAlloc, stream>>>(tq, tk, tv, t);
+  if (cudaError_t e = cudaGetLastError(); e != cudaSuccess) return e;
+  // the join goes out as a programmatic dependent launch: it waits for the pieces itself
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3(2 * sms);
+  cfg.blockDim = dim3(256);
+  cfg.stream = stream;
+  cudaLaunchAttribute attr[1];
+  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[0].val.programmaticStreamSerializationAllowed = 1;
+  cfg.attrs = attr;
+  cfg.numAttrs = 1;
+  return cudaLaunchKernelEx(&cfg, paged_join_kernel<QTiles>, t, sms);
+}
+
+// One attention of all rows over one set of page tables.
+int launch_rows(const PagedParams& p, const PagedSpace& sp, uint8_t* ws, int sms, cudaStream_t stream) {
+  // a cache expanded over heads or pages (stride 0) has no tensor map
+  const bool mapped = (p.c.head_stride > 0 || p.c.kv_heads == 1) && (p.c.page_stride > 0 || p.c.num_pages == 1) &&
+                      p.c.token_stride > 0 && (p.q_hs > 0 || p.heads == 1) && (p.q_ts > 0 || p.total_q == 1);
+  const int tiles = mapped ? q_tiles(p.max_sq, p.group) : 0;
+  if (tiles == 1) return launch_tiles<1>(p, sp, ws, sms, stream);
+  if (tiles == 2) return launch_tiles<2>(p, sp, ws, sms, stream);
+  paged_attn_kernel<<<sms * kPagedPerSm, kPagedWarps * 32, kPagedSmem, stream>>>(p);
+  return cudaGetLastError();
 }
 
 int launch_paged(const Fav4PagedArgs& a, int causal, uint8_t* ws, cudaStream_t stream) {
@@ -126,7 +202,6 @@ int launch_paged(const Fav4PagedArgs& a, int causal, uint8_t* ws, cudaStream_t s
   int rc = sm_count(&sms);
   if (rc) return rc;
   const PagedSpace sp = paged_space(a);
-  const int grid = sms * kPagedPerSm;
   PagedParams p = {};
   p.c = view_of(a.cache);
   p.q = static_cast<const __nv_bfloat16*>(a.q);
@@ -139,29 +214,31 @@ int launch_paged(const Fav4PagedArgs& a, int causal, uint8_t* ws, cudaStream_t s
   p.group = a.heads / a.cache.kv_heads;
   p.total_q = a.total_q;
   p.scale_log2 = a.scale * 1.4426950408889634f;
-  if (a.prefix_pages) {
-    // every row of the batch against the prefix, as one sequence without a mask
-    PagedParams f = p;
-    f.c.table = a.prefix_pages;
-    f.c.lens = a.prefix_len;
-    f.c.max_pages = a.max_prefix_pages;
-    f.c.batch = 1;
-    f.max_sq = a.total_q;
-    f.o32 = reinterpret_cast<float*>(ws + sp.prefix_o);
-    f.lse = reinterpret_cast<float*>(ws + sp.prefix_lse);
-    f.arrived = p.arrived + kMaxGrid;
-    paged_attn_kernel<<<grid, kPagedWarps * 32, kPagedSmem, stream>>>(f);
-    if (cudaError_t e = cudaGetLastError(); e != cudaSuccess) return e;
-    p.add_o = f.o32;
-    p.add_lse = f.lse;
-  }
   p.cu = a.cu_seqlens_q;
-  p.o = static_cast<__nv_bfloat16*>(a.o);
-  p.lse = a.lse;
   p.max_sq = a.max_sq;
   p.causal = causal;
-  paged_attn_kernel<<<grid, kPagedWarps * 32, kPagedSmem, stream>>>(p);
-  return cudaGetLastError();
+  p.o = static_cast<__nv_bfloat16*>(a.o);
+  p.lse = a.lse;
+  if (!a.prefix_pages) return launch_rows(p, sp, ws, sms, stream);
+  // every row of the batch against the prefix, as one sequence without a mask, into the workspace in FP32;
+  // then the sequences' own keys, joined with it (rows of no sequence are never written)
+  PagedParams first = p;
+  first.c.table = a.prefix_pages;
+  first.c.lens = a.prefix_len;
+  first.c.max_pages = a.max_prefix_pages;
+  first.c.batch = 1;
+  first.cu = nullptr;
+  first.max_sq = a.total_q;
+  first.causal = 0;
+  first.o = nullptr;
+  first.o32 = reinterpret_cast<float*>(ws + sp.first_o);
+  first.lse = reinterpret_cast<float*>(ws + sp.first_lse);
+  first.arrived += kMaxGrid;
+  rc = launch_rows(first, sp, ws, sms, stream);
+  if (rc) return rc;
+  p.add_o = first.o32;
+  p.add_lse = first.lse;
+  return launch_rows(p, sp, ws, sms, stream);
 }
 
 int forward_paged(const Fav4PagedArgs* a, int causal, void* workspace, size_t bytes, cudaStream_t stream,

@@ -1,0 +1,842 @@
+// Attention over the pages, 128 rows at a time (tcgen05): chunks of prompts, several drafted tokens with
+// many heads, and a whole batch against its shared prefix.
+//
+// The mathematics and the rows are paged_attn_kernel's (paged.cuh): the rows of a Q tile are `tokens`
+// consecutive new tokens times the G query heads of one K/V head, token-major, so that each K/V tile is
+// read once for up to 128 (or, with two Q tiles, 256) rows. 4 * 128 FLOP per row and key against 512
+// bytes per key: from about 130 rows on the tensor cores and the exponentials bound it, not HBM.
+//
+// A block is the warp-specialised pipeline of the contiguous kernel (attn_fwd_sm100.cuh; the TMEM
+// layout, the order of the MMAs, the softmax and its lazy rescaling are described there):
+//
+//   warps 0-3 / 4-7  softmax, correction and epilogue of Q tile 0 / 1, one row per thread
+//   warp 8           TMA: Q tiles, then the K/V ring; the lanes hold the page numbers of a tile's groups of
+//                    box_rows keys (a power of two that divides the page size) and each issues its own boxes
+//   warp 9           one thread issues every tcgen05.mma
+//   warp 10          zeroes the V rows past the end of a sequence: those slots may hold NaN, and 0 * NaN in
+//                    P V would reach the result (their scores are masked, so K needs nothing)
+//   warp 11          the schedule: pieces of work into a small ring that the other warps read
+//
+// Schedule. A unit is (sequence, K/V head, Q tiles of `block_tokens` tokens) and has as many steps as
+// 128-key tiles up to its last visible key. All units lie on one line of steps and every block takes an
+// equal stretch of it, so ragged batches, causal chunks and few rows against many keys are balanced
+// alike; the prefix sums of the steps have a closed form, so the line needs no plan and no host. A unit
+// that a boundary cuts leaves (m, l, O) per piece in the workspace, in FP32, and paged_join_kernel adds
+// them up in key order.
+#pragma once
+#include "attn_fwd_sm100.cuh"
+#include "paged.cuh"
+
+namespace fav4 {
+
+constexpr int kTileKeys = 128;
+constexpr int kPieceSlots = 4;
+constexpr uint32_t kTileSoftmaxRegs = 208;  // 128 * (2 * 208 + 88) = 384 * 168
+constexpr uint32_t kTileOtherRegs = 88;
+
+struct PagedTileParams {
+  PagedParams p;        // part_o / part_ml: [2 grid][QTiles] tiles, see below; arrived: unused
+  int4* cut;            // [grid]: the unit that block c opens and does not finish: first token, tokens, K/V head, last block (-1: none)
+  int tile_tokens;      // tokens per Q tile: 128 / group
+  int box_rows;         // keys per TMA box
+  uint32_t* status;
+  uint64_t wait_limit_ns;
+};
+
+// A stretch of one unit.
+struct Piece {
+  int token0, tokens;   // the unit's first row of Q, and how many tokens it has
+  int past;             // keys before that first token (its own position in the sequence)
+  int len, h, b;        // keys of the sequence, K/V head, sequence
+  int tile0, cnt, n;    // steps [tile0, tile0 + cnt) of n
+  int pad[7];
+};
+static_assert(sizeof(Piece) == 64, "four 16-byte words");
+
+// sum over j < n of floor((a j + c) / 128), for a, c >= 0
+__host__ __device__ __forceinline__ int64_t floor_sum128(int64_t n, int64_t a, int64_t c) {
+  int64_t m = 128, s = 0;
+  while (n > 0) {
+    s += n * (n - 1) / 2 * (a / m) + n * (c / m);
+    a %= m;
+    c %= m;
+    const int64_t y = a * n + c;
+    if (y < m) break;
+    n = y / m;
+    c = y % m;
+    const int64_t t = m;
+    m = a;
+    a = t;
+  }
+  return s;
+}
+
+__host__ __device__ __forceinline__ int steps_up_to(int64_t keys) {
+  return keys <= 0 ? 1 : static_cast<int>((keys + kTileKeys - 1) / kTileKeys);
+}
+// Steps of unit r of a sequence, and of units 0 .. r - 1.
+__host__ __device__ __forceinline__ int unit_steps(const SeqView& s, int causal, int bt, int r) {
+  const int64_t full = (static_cast<int64_t>(r) + 1) * bt;
+  const int64_t last = full < s.sq ? full : s.sq;
+  return steps_up_to(causal ? static_cast<int64_t>(s.len) - s.sq + last : s.len);
+}
+__host__ __device__ __forceinline__ int64_t units_steps(const SeqView& s, int causal, int bt, int64_t r) {
+  if (r <= 0) return 0;
+  if (!causal) return r * steps_up_to(s.len);
+  const int64_t units = (static_cast<int64_t>(s.sq) + bt - 1) / bt;
+  int64_t sum = 0;
+  if (r == units) {  // the last one ends with the sequence, the others after a whole number of bt tokens
+    sum = steps_up_to(s.len);
+    --r;
+  }
+  const int64_t past = static_cast<int64_t>(s.len) - s.sq;
+  int64_t ones = past <= kTileKeys ? (kTileKeys - past) / bt : 0;  // units that end within the first tile
+  if (ones > r) ones = r;
+  // units ones .. r - 1: ceil((past + (j + 1) bt) / 128)
+  return sum + ones + floor_sum128(r - ones, bt, past + (ones + 1) * bt + kTileKeys - 1);
+}
+__host__ __device__ __forceinline__ int64_t tile_seq_work(const SeqView& s, int causal, int bt) {
+  return s.sq == 0 ? 0 : units_steps(s, causal, bt, (static_cast<int64_t>(s.sq) + bt - 1) / bt);
+}
+
+template <int QTiles>
+struct PagedTileLayout {
+  static constexpr int kSlots = QTiles == 1 ? 3 : 2;
+  static constexpr int kSlotBytes = 2 * kTileBytes;
+  static constexpr int kQ = 0;
+  static constexpr int kKV = QTiles * kTileBytes;
+  static constexpr int kBar = kKV + kSlots * kSlotBytes;
+  static constexpr int kQFull = 0, kQEmpty = 1, kKVFull = 2, kKVEmpty = kKVFull + kSlots, kVFix = kKVEmpty + kSlots;
+  static constexpr int kSFull = kVFix + kSlots, kPFull = kSFull + 2, kOFull = kPFull + 2, kOEmpty = kOFull + 2;
+  static constexpr int kPieceFull = kOEmpty + 2, kPieceEmpty = kPieceFull + kPieceSlots;
+  static constexpr int kTeardown = kPieceEmpty + kPieceSlots;
+  static constexpr int kNumBars = kTeardown + 1;
+  static constexpr int kPieces = (kBar + kNumBars * 8 + 15) & ~15;
+  static constexpr int kMisc = kPieces + kPieceSlots * 64;  // TMEM base, abort flag, schedule scan
+  static constexpr int kScan = (kMisc + 8 + 15) & ~15;      // 12 warps' sums, then base, sequence
+  static constexpr int kBytes = kScan + 16 * 8;
+  static constexpr int kAlloc = kBytes + 1024;
+  static_assert(kAlloc <= 227 * 1024, "shared memory budget");
+};
+
+// Rows of one tile in the workspace, as the softmax threads (one row each) write them: 4-column piece c of
+// row r at float4 index c * 128 + r, so that a warp's stores and loads are whole lines.
+__device__ __forceinline__ int64_t part_tile(int slot, int qtiles, int i) { return static_cast<int64_t>(slot) * qtiles + i; }
+
+template <int QTiles>
+__global__ void __launch_bounds__(384, 1)
+    paged_tile_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant__ CUtensorMap tm_k,
+                      const __grid_constant__ CUtensorMap tm_v, const __grid_constant__ PagedTileParams tp) {
+  using L = PagedTileLayout<QTiles>;
+  constexpr int Slots = L::kSlots;
+  constexpr int KA = QTiles == 1 ? 2 : 1;  // S runs this many steps ahead of P V
+  const PagedParams& p = tp.p;
+  extern __shared__ uint8_t smem_raw[];
+  uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
+  const uint32_t sbase = smem_addr(smem);
+  const uint32_t bar0 = sbase + L::kBar;
+  auto bar = [&](int slot) -> uint32_t { return bar0 + 8u * slot; };
+  uint32_t* tmem_holder = reinterpret_cast<uint32_t*>(smem + L::kMisc);
+  volatile uint32_t* abort_flag = reinterpret_cast<volatile uint32_t*>(smem + L::kMisc + 4);
+  int64_t* scan = reinterpret_cast<int64_t*>(smem + L::kScan);
+  Piece* pieces = reinterpret_cast<Piece*>(smem + L::kPieces);
+
+  const int warp = threadIdx.x / 32;
+  const int lane = threadIdx.x % 32;
+  WaitCtl ctl{abort_flag, tp.status, tp.wait_limit_ns};
+
+  if (threadIdx.x == 0) {
+    *abort_flag = 0u;
+    mbar_init(bar(L::kQFull), 1);
+    mbar_init(bar(L::kQEmpty), 1);
+    for (int s = 0; s < Slots; ++s) {
+      mbar_init(bar(L::kKVFull + s), 1);
+      mbar_init(bar(L::kKVEmpty + s), 2);  // the MMAs that read it, and warp 10
+      mbar_init(bar(L::kVFix + s), 1);
+    }
+    for (int i = 0; i < 2; ++i) {
+      mbar_init(bar(L::kSFull + i), 1);
+      mbar_init(bar(L::kPFull + i), 4);
+      mbar_init(bar(L::kOFull + i), 1);
+      mbar_init(bar(L::kOEmpty + i), 4);
+    }
+    for (int s = 0; s < kPieceSlots; ++s) {
+      mbar_init(bar(L::kPieceFull + s), 1);
+      mbar_init(bar(L::kPieceEmpty + s), 3 + 4 * QTiles);  // load, MMA and V warps, softmax warps
+    }
+    mbar_init(bar(L::kTeardown), 1);
+    fence_mbar_init();
+  }
+  if (warp == 8 && lane == 0) {
+    tma_prefetch_desc(&tm_q);
+    tma_prefetch_desc(&tm_k);
+    tma_prefetch_desc(&tm_v);
+  }
+  if (warp == 9) {
+    tmem_alloc(smem_addr(tmem_holder), 512);
+    tmem_relinquish();
+  }
+  asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
+
+  // ---- this block's stretch of the line of steps, and the sequence that it begins in ----
+  const int bt = tp.tile_tokens * QTiles;
+  int64_t total = 0, per = 1, begin = 0;
+  for (int pass = 0; pass < 2; ++pass) {
+    int64_t base = 0;
+    for (int b0 = 0; b0 < p.c.batch; b0 += 384) {
+      const int b = b0 + threadIdx.x;
+      int64_t v = 0;
+      if (b < p.c.batch) v = tile_seq_work(seq_view(p.c, p.cu, p.total_q, p.max_sq, b), p.causal, bt) * p.c.kv_heads;
+      const int64_t mine = v;
+#pragma unroll
+      for (int o = 1; o < 32; o *= 2) {
+        const int64_t up = __shfl_up_sync(0xffffffffu, v, o);
+        if (lane >= o) v += up;
+      }
+      if (lane == 31) scan[warp] = v;
+      __syncthreads();
+      int64_t sum = 0;
+      for (int w = 0; w < 12; ++w) {
+        if (w < warp) v += scan[w];
+        sum += scan[w];
+      }
+      if (p.c.batch <= 384) {  // one step sees the whole batch
+        total = sum;
+        per = max((total + gridDim.x - 1) / gridDim.x, int64_t(1));
+        begin = blockIdx.x * per;
+        pass = 1;
+      }
+      if (pass == 1 && base + v - mine <= begin && begin < base + v) {
+        scan[12] = base + v - mine;
+        scan[13] = b;
+      }
+      base += sum;
+      __syncthreads();
+    }
+    if (pass == 0) {
+      total = base;
+      per = max((total + gridDim.x - 1) / gridDim.x, int64_t(1));
+      begin = blockIdx.x * per;
+    }
+  }
+  const int64_t end = min(total, begin + per);
+
+  tc_fence_before();
+  __syncthreads();
+  tc_fence_after();
+  const uint32_t tmem = *tmem_holder;
+
+  // Reads the next piece; every warp that calls it does so converged and releases the slot at once.
+  int piece_at = 0;
+  auto next_piece = [&](Piece* out) -> bool {
+    const int s = piece_at % kPieceSlots;
+    if (!warp_wait(bar(L::kPieceFull + s), (piece_at / kPieceSlots) & 1u, ctl, kStatusTimeoutLoad)) return false;
+    const int4* src = reinterpret_cast<const int4*>(pieces + s);
+    int4 w0 = src[0], w1 = src[1], w2 = src[2];
+    out->token0 = w0.x; out->tokens = w0.y; out->past = w0.z; out->len = w0.w;
+    out->h = w1.x; out->b = w1.y; out->tile0 = w1.z; out->cnt = w1.w;
+    out->n = w2.x;
+    __syncwarp();
+    if (lane == 0) mbar_arrive(bar(L::kPieceEmpty + s));
+    ++piece_at;
+    return out->cnt > 0;
+  };
+  // Steps of Q tile i within the piece (0: none of its rows sees a key there).
+  auto tile_steps = [&](const Piece& w, int i) -> int {
+    const int t0 = i * tp.tile_tokens;
+    if (t0 >= w.tokens) return 0;
+    int64_t keys = w.len;
+    if (p.causal) keys = min(keys, static_cast<int64_t>(w.past) + min(w.tokens, t0 + tp.tile_tokens));
+    if (keys <= 0) return 0;
+    const int n = static_cast<int>((keys + kTileKeys - 1) / kTileKeys);
+    return max(min(n - w.tile0, w.cnt), 0);
+  };
+
+  static_assert(128 * (2 * kTileSoftmaxRegs + kTileOtherRegs) <= 384 * kLaunchRegs, "register split exceeds the launch");
+  static_assert(128 * (kSoftmaxRegs1 + kOtherRegs + kOtherRegs1) <= 384 * kLaunchRegs, "register split exceeds the launch");
+
+  if (warp >= 8) {
+    regs_release<(QTiles == 1 ? kOtherRegs1 : kTileOtherRegs)>();
+    if (warp == 8) {
+      // ============================ TMA producer ============================
+      const uint64_t pol_kv = policy_evict_last();
+      const uint64_t pol_q = policy_evict_first();
+      Ring ring;
+      LoadState<true> st;
+      bool ok = true;
+      Piece w;
+      const int R = tp.box_rows, groups = kTileKeys / R;
+      const uint32_t q_box = static_cast<uint32_t>(tp.tile_tokens) * p.group * 128u;
+      while (ok && next_piece(&w)) {
+        const int n0 = tile_steps(w, 0), n1 = QTiles > 1 ? tile_steps(w, 1) : 0;
+        const int N = max(n0, n1);
+        if (N == 0) continue;
+        if (!warp_wait(bar(L::kQEmpty), st.q_empty(), ctl, kStatusTimeoutLoad)) { ok = false; break; }
+        st.flip_q_empty();
+        if (lane == 0) {
+          mbar_arrive_expect_tx(bar(L::kQFull), ((n0 > 0 ? 1 : 0) + (n1 > 0 ? 1 : 0)) * 2 * q_box);
+          for (int i = 0; i < QTiles; ++i) {
+            if ((i == 0 ? n0 : n1) == 0) continue;
+            const uint32_t dst = sbase + L::kQ + i * kTileBytes;
+            const int row = w.token0 + i * tp.tile_tokens;
+            tma_load_3d(dst, &tm_q, bar(L::kQFull), 0, w.h * p.group, row, pol_q);
+            tma_load_3d(dst + kBoxBytes, &tm_q, bar(L::kQFull), 64, w.h * p.group, row, pol_q);
+          }
+        }
+        __syncwarp();
+        // Lane g < groups has the page of keys [128 t + g R, + R) of the K tile to come; lane 16 + g the same of
+        // the V tile, which follows its K tile by KA groups of the ring.
+        const int* table = p.c.table + w.b * p.c.table_stride;
+        const int grp = lane % 16;
+        auto page_of = [&](int j) -> int {
+          const int64_t key = static_cast<int64_t>(w.tile0 + j) * kTileKeys + grp * R;
+          if (grp >= groups || j >= N || key >= w.len) return 0;
+          return min(max(__ldg(table + key / p.c.page_size), 0), p.c.num_pages - 1);
+        };
+        const int lead = lane < 16 ? KA : 0;  // K lanes look at tile g + KA, V lanes at tile g
+        int page = page_of(lead - KA < 0 ? N : lead - KA);
+        for (int g = -KA; g < N && ok; ++g) {
+          const bool has_v = g >= 0, has_k = g + KA < N;
+          const int j = g + lead;
+          const int page_next = g + 1 + lead >= 0 ? page_of(g + 1 + lead) : 0;
+          if (KA > 1 && !has_v && !has_k) { page = page_next; continue; }
+          if (!warp_wait(bar(L::kKVEmpty + ring.stage), ring.phase ^ 1u, ctl, kStatusTimeoutLoad)) { ok = false; break; }
+          const uint32_t fb = bar(L::kKVFull + ring.stage);
+          auto tile_bytes = [&](int t) -> uint32_t {  // whole groups up to the last key
+            const int64_t left = static_cast<int64_t>(w.len) - static_cast<int64_t>(w.tile0 + t) * kTileKeys;
+            return left >= kTileKeys ? kTileBytes : static_cast<uint32_t>((left + R - 1) / R * R) * 256u;
+          };
+          if (lane == 0)
+            mbar_arrive_expect_tx(fb, (has_v ? tile_bytes(g) : 0u) + (has_k ? tile_bytes(g + KA) : 0u));
+          st.arm(ring.stage, ring.phase);
+          __syncwarp();
+          const int64_t key = static_cast<int64_t>(w.tile0 + j) * kTileKeys + grp * R;
+          if (grp < groups && j >= 0 && j < N && key < w.len) {
+            const uint32_t dst = sbase + L::kKV + ring.stage * L::kSlotBytes + (lane < 16 ? kTileBytes : 0) + grp * R * 128;
+            const CUtensorMap* map = lane < 16 ? &tm_k : &tm_v;
+            const int slot = static_cast<int>(key % p.c.page_size);
+            tma_load_4d(dst, map, fb, 0, w.h, slot, page, pol_kv);
+            tma_load_4d(dst + kBoxBytes, map, fb, 64, w.h, slot, page, pol_kv);
+          }
+          __syncwarp();
+          page = page_next;
+          ring.advance<Slots>();
+        }
+      }
+      if (*abort_flag) {
+        // Let every copy this warp issued land before the block exits.
+        volatile uint32_t no_abort = 0;
+        WaitCtl drain{&no_abort, tp.status, tp.wait_limit_ns};
+        for (int s = 0; s < Slots; ++s)
+          if (st.was_armed(s)) mbar_wait(bar(L::kKVFull + s), st.armed_parity(s), drain, kStatusTimeoutDrain);
+      }
+      __syncwarp();
+    } else if (warp == 9) {
+      // ============================= MMA issuer =============================
+      constexpr uint32_t idesc_qk = make_idesc_bf16(kBlockM, kTileKeys, false);
+      constexpr uint32_t idesc_pv = make_idesc_bf16(kBlockM, kHeadDim, true);
+      Ring ring;
+      MmaParities<true> par;
+      uint32_t fix_par = 0;  // bit s: parity of the V fix barrier of slot s
+      bool ok = true;
+      const uint64_t dk = make_sdesc_sw128(sbase, 16, 1024);
+      const uint64_t dv = make_sdesc_sw128(sbase, kBoxBytes, 1024);
+      const uint32_t k_lo = static_cast<uint32_t>(dk), k_hi = static_cast<uint32_t>(dk >> 32);
+      const uint32_t v_lo = static_cast<uint32_t>(dv), v_hi = static_cast<uint32_t>(dv >> 32);
+      // S = Q_i K^T into TMEM columns 128 s; O_i += P V, P at columns 128 s
+      auto issue_s = [&](int i, int s, int slot) {
+        const uint32_t qa = k_lo + ((L::kQ + i * kTileBytes) >> 4);
+        const uint32_t ka = k_lo + ((L::kKV + slot * L::kSlotBytes + kTileBytes) >> 4);
+        const uint32_t d = tmem + s * 128;
+#pragma unroll
+        for (int k = 0; k < kHeadDim / 16; ++k) {
+          const uint32_t off = ((k / 4) * kBoxBytes + (k % 4) * 32) >> 4;
+          umma_ss_w(d, qa + off, k_hi, ka + off, k_hi, idesc_qk, k > 0 ? 1u : 0u);
+        }
+        tc_commit(bar(L::kSFull + s));
+      };
+      auto issue_pv = [&](int i, int s, int slot, bool acc) {
+        const uint32_t va = v_lo + ((L::kKV + slot * L::kSlotBytes) >> 4);
+        const uint32_t d = tmem + 256 + i * 128, pa = tmem + s * 128;
+        umma_ts_w(d, pa, va, v_hi, idesc_pv, acc ? 1u : 0u);
+#pragma unroll
+        for (int k = 1; k < kTileKeys / 16; ++k) umma_ts_w(d, pa + k * 8, va + ((k * 2048) >> 4), v_hi, idesc_pv, 1u);
+      };
+      Piece w;
+      while (ok && next_piece(&w)) {
+        const int n0 = tile_steps(w, 0), n1 = QTiles > 1 ? tile_steps(w, 1) : 0;
+        const int N = max(n0, n1);
+        if (N == 0) continue;
+        if (lane == 0) {
+          // the last V tile has rows past the end of the sequence
+          const bool ragged = static_cast<int64_t>(w.tile0 + N) * kTileKeys > w.len;
+          auto wait_fix = [&](int slot) -> bool {
+            if (!mbar_wait(bar(L::kVFix + slot), (fix_par >> slot) & 1u, ctl, kStatusTimeoutMma)) return false;
+            fix_par ^= 1u << slot;
+            return true;
+          };
+          if (!mbar_wait(bar(L::kQFull), par.q_full(), ctl, kStatusTimeoutMma)) ok = false;
+          par.flip_q_full();
+          if constexpr (QTiles == 1) {
+            // S buffers j % 2; every P V is committed to pv_done (the o_full barrier of the second tile)
+            for (int pb = 0; pb < 2 && pb < N && ok; ++pb) {
+              if (!mbar_wait(bar(L::kKVFull + ring.stage), ring.phase, ctl, kStatusTimeoutMma)) { ok = false; break; }
+              tc_fence_after();
+              issue_s(0, pb, ring.stage);
+              tc_commit(bar(L::kKVEmpty + ring.stage));
+              ring.advance<Slots>();
+            }
+            if (N <= 2 && ok) tc_commit(bar(L::kQEmpty));
+            if (ok && !mbar_wait(bar(L::kKVFull + ring.stage), ring.phase, ctl, kStatusTimeoutMma)) ok = false;
+            for (int j = 0; j < N && ok; ++j) {
+              const int b = j & 1, cur = ring.stage;
+              if (!mbar_wait(bar(L::kPFull + b), par.p_full(b), ctl, kStatusTimeoutMma)) { ok = false; break; }
+              par.flip_p_full(b);
+              if (j == 0) {
+                if (!mbar_wait(bar(L::kOEmpty), par.o_empty(0), ctl, kStatusTimeoutMma)) { ok = false; break; }
+                par.flip_o_empty(0);
+              }
+              if (ragged && j + 1 == N && !wait_fix(cur)) { ok = false; break; }
+              tc_fence_after();
+              issue_pv(0, b, cur, j > 0);
+              tc_commit(bar(L::kOFull + 1));
+              if (j + 1 == N) tc_commit(bar(L::kOFull));
+              if (j + 2 < N) issue_s(0, b, cur);
+              tc_commit(bar(L::kKVEmpty + cur));
+              if (j + 3 == N) tc_commit(bar(L::kQEmpty));
+              ring.advance<Slots>();
+              if (j + 1 < N && !mbar_wait(bar(L::kKVFull + ring.stage), ring.phase, ctl, kStatusTimeoutMma)) {
+                ok = false;
+                break;
+              }
+            }
+          } else {
+            if (ok && !mbar_wait(bar(L::kKVFull + ring.stage), ring.phase, ctl, kStatusTimeoutMma)) ok = false;
+            if (ok) {
+              tc_fence_after();
+              if (n0 > 0) issue_s(0, 0, ring.stage);
+              if (n1 > 0) issue_s(1, 1, ring.stage);
+              tc_commit(bar(L::kKVEmpty + ring.stage));
+              if (N == 1) tc_commit(bar(L::kQEmpty));
+              ring.advance<Slots>();
+              if (!mbar_wait(bar(L::kKVFull + ring.stage), ring.phase, ctl, kStatusTimeoutMma)) ok = false;
+            }
+            for (int j = 0; j < N && ok; ++j) {
+              const int cur = ring.stage;
+              Ring nxt = ring;
+              nxt.advance<Slots>();
+              if (ragged && j + 1 == N && !wait_fix(cur)) { ok = false; break; }
+#pragma unroll
+              for (int i = 0; i < QTiles; ++i) {
+                const int ni = i == 0 ? n0 : n1;
+                if (j < ni && ok) {
+                  if (!mbar_wait(bar(L::kPFull + i), par.p_full(i), ctl, kStatusTimeoutMma)) { ok = false; continue; }
+                  par.flip_p_full(i);
+                  if (j == 0) {
+                    if (!mbar_wait(bar(L::kOEmpty + i), par.o_empty(i), ctl, kStatusTimeoutMma)) { ok = false; continue; }
+                    par.flip_o_empty(i);
+                  }
+                  tc_fence_after();
+                  issue_pv(i, i, cur, j > 0);
+                  if (j + 1 == ni) tc_commit(bar(L::kOFull + i));
+                }
+                if (i == QTiles - 1 && j + 1 < N && ok) {
+                  if (!mbar_wait(bar(L::kKVFull + nxt.stage), nxt.phase, ctl, kStatusTimeoutMma)) { ok = false; continue; }
+                }
+                if (j + 1 < ni && ok) issue_s(i, i, cur);
+              }
+              if (!ok) break;
+              tc_commit(bar(L::kKVEmpty + cur));
+              if (j + 2 == N) tc_commit(bar(L::kQEmpty));
+              ring = nxt;
+            }
+          }
+        }
+        ok = __all_sync(0xffffffffu, ok);
+      }
+      if (lane == 0) {
+        // Every MMA this thread issued has finished once this barrier flips.
+        tc_commit(bar(L::kTeardown));
+        volatile uint32_t no_abort = 0;
+        WaitCtl drain{&no_abort, tp.status, tp.wait_limit_ns};
+        mbar_wait(bar(L::kTeardown), 0, drain, kStatusTimeoutDrain);
+      }
+      __syncwarp();
+    } else if (warp == 10) {
+      // ================== zeros for V rows past the end ==================
+      // It follows every group of the ring (and releases each, so that it stays within one round of it).
+      Ring ring;
+      bool ok = true;
+      Piece w;
+      while (ok && next_piece(&w)) {
+        const int N = max(tile_steps(w, 0), QTiles > 1 ? tile_steps(w, 1) : 0);
+        if (N == 0) continue;
+        const int64_t first = static_cast<int64_t>(w.tile0 + N - 1) * kTileKeys;  // of the last V tile
+        const int row = first + kTileKeys > w.len ? static_cast<int>(w.len - first) : kTileKeys;
+        for (int left = N + min(KA, N); left > 0; --left) {
+          if (!warp_wait(bar(L::kKVFull + ring.stage), ring.phase, ctl, kStatusTimeoutLoad)) { ok = false; break; }
+          if (left == 1 && row < kTileKeys) {
+            uint8_t* v = smem + L::kKV + ring.stage * L::kSlotBytes;
+            for (int x = row * 8 + lane; x < kTileKeys * 8; x += 32) {
+              reinterpret_cast<uint4*>(v)[x] = make_uint4(0u, 0u, 0u, 0u);
+              reinterpret_cast<uint4*>(v + kBoxBytes)[x] = make_uint4(0u, 0u, 0u, 0u);
+            }
+            fence_proxy_async_smem();
+            __syncwarp();
+            if (lane == 0) mbar_arrive(bar(L::kVFix + ring.stage));
+          }
+          if (lane == 0) mbar_arrive(bar(L::kKVEmpty + ring.stage));
+          ring.advance<Slots>();
+        }
+      }
+    } else if (lane == 0) {
+      // ============================== schedule ==============================
+      int4 cut = make_int4(0, 0, 0, -1);
+      int out = 0;
+      auto slot_free = [&]() -> bool {
+        const int s = out % kPieceSlots;
+        return mbar_wait(bar(L::kPieceEmpty + s), ((out / kPieceSlots) & 1u) ^ 1u, ctl, kStatusTimeoutLoad);
+      };
+      auto put = [&](const Piece& w) {
+        const int s = out % kPieceSlots;
+        int4* dst = reinterpret_cast<int4*>(pieces + s);
+        dst[0] = make_int4(w.token0, w.tokens, w.past, w.len);
+        dst[1] = make_int4(w.h, w.b, w.tile0, w.cnt);
+        dst[2] = make_int4(w.n, 0, 0, 0);
+        mbar_arrive(bar(L::kPieceFull + s));  // releases the writes above
+        ++out;
+      };
+      bool ok = true;
+      if (begin < end) {
+        int64_t base = scan[12];
+        int b = static_cast<int>(scan[13]);
+        int64_t pos = begin;
+        while (pos < end && ok) {
+          const SeqView s = seq_view(p.c, p.cu, p.total_q, p.max_sq, b);
+          const int64_t head_work = tile_seq_work(s, p.causal, bt);
+          const int units = (s.sq + bt - 1) / bt;
+          const int64_t stop = min(end, base + head_work * p.c.kv_heads);
+          if (pos < stop) {
+            int h = static_cast<int>((pos - base) / head_work);
+            // the unit that holds `pos`: the last r whose earlier units end at or before it
+            const int64_t x = pos - base - h * head_work;
+            int lo = 0, hi = units - 1;
+            while (lo < hi) {
+              const int mid = (lo + hi + 1) / 2;
+              if (units_steps(s, p.causal, bt, mid) <= x) lo = mid;
+              else hi = mid - 1;
+            }
+            int r = lo;
+            int64_t first = base + h * head_work + units_steps(s, p.causal, bt, r);  // the unit's place on the line
+            while (pos < stop) {
+              Piece w;
+              w.n = unit_steps(s, p.causal, bt, r);
+              w.token0 = s.q0 + r * bt;
+              w.tokens = min(bt, s.sq - r * bt);
+              w.past = s.len - s.sq + r * bt;
+              w.len = s.len;
+              w.h = h;
+              w.b = b;
+              w.tile0 = static_cast<int>(pos - first);
+              w.cnt = static_cast<int>(min(static_cast<int64_t>(w.n - w.tile0), end - pos));
+              if (!slot_free()) { ok = false; break; }
+              put(w);
+              if (w.tile0 == 0 && w.cnt < w.n)
+                cut = make_int4(w.token0, w.tokens, h, static_cast<int>((first + w.n - 1) / per));
+              pos += w.cnt;
+              first += w.n;
+              if (++r == units) {
+                r = 0;
+                ++h;
+              }
+            }
+          }
+          base += head_work * p.c.kv_heads;
+          ++b;
+        }
+      }
+      tp.cut[blockIdx.x] = cut;
+      if (ok && slot_free()) {
+        Piece w = {};
+        put(w);  // cnt = 0: no more
+      }
+    }
+  } else if (warp < 4 * QTiles) {
+    // ============================== softmax ===============================
+    regs_claim<(QTiles == 1 ? kSoftmaxRegs1 : kTileSoftmaxRegs)>();
+    const int i = warp / 4;
+    const int row = (warp % 4) * 32 + lane;
+    const uint32_t lane_off = static_cast<uint32_t>((warp % 4) * 32) << 16;
+    const uint32_t t_s0 = tmem + lane_off + i * 128;
+    const uint32_t t_o = tmem + lane_off + 256 + i * 128;
+    uint32_t s_par = 0, o_full_par = 0, pv_seen = 0;
+    const float scale_log2 = p.scale_log2;
+    const int row_token = row / p.group;                    // token of this row within the Q tile
+    const int row_head = row - row_token * p.group;
+    bool ok = true;
+    Piece w;
+    while (ok && next_piece(&w)) {
+      const int t0 = i * tp.tile_tokens;
+      if (t0 >= w.tokens) continue;  // no rows in this Q tile
+      const int ni = tile_steps(w, i);
+      const bool live = row_token < tp.tile_tokens && t0 + row_token < w.tokens;
+      const int first_lim = p.causal ? w.past + t0 : w.len - 1;                 // last visible key of the tile's first row
+      const int lim_row = p.causal ? w.past + t0 + row_token : w.len - 1;       // and of this one
+      float m = -INFINITY, l = 0.f;
+      for (int j = 0; j < ni; ++j) {
+        const int sb = QTiles == 1 ? (j & 1) : i;
+        const uint32_t t_s = t_s0 + (QTiles == 1 ? sb * 128 : 0);
+        const uint32_t s_bit = QTiles == 1 ? 1u << sb : 1u;
+        if (!warp_wait(bar(L::kSFull + sb), (s_par & s_bit) ? 1u : 0u, ctl, kStatusTimeoutSoftmax)) { ok = false; break; }
+        s_par ^= s_bit;
+        tc_fence_after();
+        uint32_t sr[4][32];
+#pragma unroll
+        for (int c = 0; c < 4; ++c) tmem_ld32(t_s + c * 32, sr[c]);
+        tmem_ld_wait();
+        float s[128];
+#pragma unroll
+        for (int c = 0; c < 128; ++c) s[c] = __uint_as_float(sr[c / 32][c % 32]);
+        const int col0 = (w.tile0 + j) * kTileKeys;
+        const bool masked = col0 + kTileKeys - 1 > min(first_lim, w.len - 1);
+        if (masked) {
+          const int lim = min(lim_row, w.len - 1) - col0;
+#pragma unroll
+          for (int c = 0; c < 128; ++c) s[c] = c > lim ? -INFINITY : s[c];
+        }
+        float mx0 = fmax3(s[0], s[1], s[2]), mx1 = fmax3(s[3], s[4], s[5]);
+        float mx2 = fmax3(s[6], s[7], s[8]), mx3 = fmax3(s[9], s[10], s[11]);
+#pragma unroll
+        for (int c = 12; c < 124; c += 8) {
+          mx0 = fmax3(mx0, s[c], s[c + 1]);
+          mx1 = fmax3(mx1, s[c + 2], s[c + 3]);
+          mx2 = fmax3(mx2, s[c + 4], s[c + 5]);
+          mx3 = fmax3(mx3, s[c + 6], s[c + 7]);
+        }
+        mx0 = fmax3(mx0, s[124], s[125]);
+        mx1 = fmax3(mx1, s[126], s[127]);
+        const float mx = fmax3(fmaxf(mx0, mx1), mx2, mx3) * scale_log2;
+        const float cand = fmaxf(m, mx);
+        const bool update = (j == 0) || (cand > m + kRescaleThreshold);
+        const float m_new = update ? cand : m;
+        const bool rescale = (j > 0) && __any_sync(0xffffffffu, update);
+        const float alpha = rescale ? ((m_new == -INFINITY) ? 1.f : ex2_mufu(m - m_new)) : 1.f;
+        m = m_new;
+        const float mb = (m == -INFINITY) ? 0.f : m;
+        const float rowsum = masked ? exp_pack_store<0, true>(s, scale_log2, mb, t_s)
+                                    : exp_pack_store<0, false>(s, scale_log2, mb, t_s);
+        l = l * alpha + rowsum;
+        if (rescale) {
+          if (QTiles == 1) {  // S runs two steps ahead: P V of the step before may still be at work on O
+            if (!warp_wait(bar(L::kOFull + 1), (pv_seen + j - 1) & 1u, ctl, kStatusTimeoutSoftmax)) { ok = false; break; }
+            tc_fence_after();
+          }
+          const float2 a2 = make_float2(alpha, alpha);
+#pragma unroll 1
+          for (int c = 0; c < 4; ++c) {
+            uint32_t orow[32];
+            tmem_ld32(t_o + c * 32, orow);
+            tmem_ld_wait();
+#pragma unroll
+            for (int e = 0; e < 32; e += 2) {
+              const float2 v = __fmul2_rn(make_float2(__uint_as_float(orow[e]), __uint_as_float(orow[e + 1])), a2);
+              orow[e] = __float_as_uint(v.x);
+              orow[e + 1] = __float_as_uint(v.y);
+            }
+            tmem_st32(t_o + c * 32, orow);
+          }
+        }
+        tmem_st_wait();
+        tc_fence_before();
+        __syncwarp();
+        if (lane == 0) mbar_arrive(bar(L::kPFull + sb));
+      }
+      if (!ok) break;
+      pv_seen += ni;
+      // ------------------------------ epilogue ------------------------------
+      uint32_t oall[4][32];
+      if (ni > 0) {
+        if (!warp_wait(bar(L::kOFull + i), o_full_par, ctl, kStatusTimeoutSoftmax)) { ok = false; break; }
+        o_full_par ^= 1u;
+        tc_fence_after();
+#pragma unroll
+        for (int c = 0; c < 4; ++c) tmem_ld32(t_o + c * 32, oall[c]);
+        tmem_ld_wait();
+        tc_fence_before();
+        __syncwarp();
+        if (lane == 0) mbar_arrive(bar(L::kOEmpty + i));
+      } else {
+#pragma unroll
+        for (int c = 0; c < 128; ++c) oall[c / 32][c % 32] = 0u;
+      }
+      auto ov = [&](int c) -> float { return __uint_as_float(oall[c / 32][c % 32]); };
+      if (w.cnt < w.n) {  // a piece: (m, l, O) to the workspace
+        const int64_t tile = part_tile(2 * blockIdx.x + (w.tile0 == 0 ? 1 : 0), QTiles, i);
+        float4* dst = reinterpret_cast<float4*>(p.part_o) + tile * 4096 + row;
+#pragma unroll
+        for (int c = 0; c < 32; ++c) dst[c * 128] = make_float4(ov(4 * c), ov(4 * c + 1), ov(4 * c + 2), ov(4 * c + 3));
+        reinterpret_cast<float2*>(p.part_ml)[tile * 128 + row] = make_float2(m, l);
+      } else if (live) {
+        const int64_t token = w.token0 + t0 + row_token;
+        const int head = w.h * p.group + row_head;
+        const int64_t orow = token * p.heads + head, lse_at = static_cast<int64_t>(head) * p.total_q + token;
+        float a = 1.f, x = 0.f;
+        if (p.add_o != nullptr) {  // the other result of this row, joined in
+          asm volatile("griddepcontrol.wait;" ::: "memory");
+          const float other = __ldcg(p.add_lse + lse_at) * 1.4426950408889634f;
+          const float top = fmaxf(m, other);
+          if (top != -INFINITY) {
+            a = exp2f(m - top);
+            x = exp2f(other - top);
+            l = l * a + x;
+            m = top;
+          }
+        }
+        const float inv = l == 0.f ? 0.f : 1.f / l;
+        a *= inv;
+        x *= inv;
+        const float4* add = reinterpret_cast<const float4*>(p.add_o + orow * 128);
+#pragma unroll
+        for (int c = 0; c < 32; c += 2) {
+          float4 u = make_float4(ov(4 * c) * a, ov(4 * c + 1) * a, ov(4 * c + 2) * a, ov(4 * c + 3) * a);
+          float4 v = make_float4(ov(4 * c + 4) * a, ov(4 * c + 5) * a, ov(4 * c + 6) * a, ov(4 * c + 7) * a);
+          if (p.add_o != nullptr) {
+            const float4 e = __ldcg(add + c), f = __ldcg(add + c + 1);
+            u = make_float4(fmaf(e.x, x, u.x), fmaf(e.y, x, u.y), fmaf(e.z, x, u.z), fmaf(e.w, x, u.w));
+            v = make_float4(fmaf(f.x, x, v.x), fmaf(f.y, x, v.y), fmaf(f.z, x, v.z), fmaf(f.w, x, v.w));
+          }
+          if (p.o != nullptr) {
+            *reinterpret_cast<uint4*>(p.o + orow * 128 + c * 4) =
+                make_uint4(pack_bf16x2(u.x, u.y), pack_bf16x2(u.z, u.w), pack_bf16x2(v.x, v.y), pack_bf16x2(v.z, v.w));
+          } else {
+            reinterpret_cast<float4*>(p.o32 + orow * 128)[c] = u;
+            reinterpret_cast<float4*>(p.o32 + orow * 128)[c + 1] = v;
+          }
+        }
+        if (p.lse != nullptr) p.lse[lse_at] = l == 0.f ? -INFINITY : m * kLn2 + logf(l);
+      }
+    }
+  } else {
+    regs_release<kOtherRegs>();  // warps 4-7 when QTiles == 1
+  }
+
+  tc_fence_before();
+  __syncthreads();
+  if (warp == 9) {
+    tc_fence_after();
+    tmem_dealloc(tmem, 512);
+  }
+}
+
+// Adds up the pieces of the units that paged_tile_kernel cut, in key order: O = sum 2^(m_c - M) O_c / L,
+// M = max m_c, L = sum 2^(m_c - M) l_c. Reads each piece once and writes each row once, so L2 bandwidth
+// bounds it; the work items are (unit, Q tile, 4 columns), 128 rows wide, the pieces of each in two
+// halves, so that two units cut into 64 pieces still occupy every SM.
+template <int QTiles>
+__global__ void __launch_bounds__(256) paged_join_kernel(const __grid_constant__ PagedTileParams tp, int blocks) {
+  constexpr int kMaxCuts = 256;
+  __shared__ int4 cuts[kMaxCuts];
+  __shared__ int first_block[kMaxCuts];
+  __shared__ int warp_cuts[kMaxCuts / 32];
+  __shared__ float4 half_o[128];
+  __shared__ float2 half_ml[128];
+  const PagedParams& p = tp.p;
+  asm volatile("griddepcontrol.wait;" ::: "memory");
+  // the cut units, numbered alike in every block: by the block that opens them (blocks <= kMaxCuts threads)
+  const int4 mine = static_cast<int>(threadIdx.x) < blocks ? __ldcg(tp.cut + threadIdx.x) : make_int4(0, 0, 0, -1);
+  const uint32_t opens = __ballot_sync(0xffffffffu, mine.w >= 0);
+  if (threadIdx.x % 32 == 0) warp_cuts[threadIdx.x / 32] = __popc(opens);
+  __syncthreads();
+  int at = __popc(opens & ((1u << (threadIdx.x % 32)) - 1)), count = 0;
+#pragma unroll
+  for (int w = 0; w < kMaxCuts / 32; ++w) {
+    if (w < static_cast<int>(threadIdx.x / 32)) at += warp_cuts[w];
+    count += warp_cuts[w];
+  }
+  if (mine.w >= 0) {
+    cuts[at] = mine;
+    first_block[at] = threadIdx.x;
+  }
+  __syncthreads();
+  const int row = threadIdx.x % 128, half = threadIdx.x / 128;
+  const int row_token = row / p.group, row_head = row - row_token * p.group;
+  const float4* part_o = reinterpret_cast<const float4*>(p.part_o);
+  const float2* part_ml = reinterpret_cast<const float2*>(p.part_ml);
+  const int items = count * QTiles * 32;
+  for (int item = blockIdx.x; item < items; item += gridDim.x) {
+    const int u = item / (QTiles * 32), i = item / 32 % QTiles, col = item % 32;
+    const int4 c = cuts[u];
+    const int t0 = i * tp.tile_tokens;
+    if (t0 >= c.y) continue;  // block-uniform
+    const int c0 = first_block[u], parts = c.w - c0 + 1;
+    const int mid = (parts + 1) / 2, from = half ? mid : 0, to = half ? parts : mid;
+    auto tile = [&](int x) { return part_tile(2 * (c0 + x) + (x == 0 ? 1 : 0), QTiles, i); };
+    float m = -INFINITY, l = 0.f;
+    float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
+    for (int x0 = from; x0 < to; x0 += 8) {
+      float2 ml[8];
+      float4 o[8];
+#pragma unroll
+      for (int x = 0; x < 8; ++x) {
+        if (x0 + x < to) {
+          ml[x] = __ldcg(part_ml + tile(x0 + x) * 128 + row);
+          o[x] = __ldcg(part_o + tile(x0 + x) * 4096 + col * 128 + row);
+        } else {
+          ml[x] = make_float2(-INFINITY, 0.f);
+          o[x] = make_float4(0.f, 0.f, 0.f, 0.f);
+        }
+      }
+      float top = m;
+#pragma unroll
+      for (int x = 0; x < 8; ++x) top = fmaxf(top, ml[x].x);
+      if (top != -INFINITY) {
+        const float a = exp2f(m - top);
+        acc = make_float4(acc.x * a, acc.y * a, acc.z * a, acc.w * a);
+        l *= a;
+        m = top;
+#pragma unroll
+        for (int x = 0; x < 8; ++x) {
+          const float b = exp2f(ml[x].x - top);
+          acc = make_float4(fmaf(o[x].x, b, acc.x), fmaf(o[x].y, b, acc.y), fmaf(o[x].z, b, acc.z), fmaf(o[x].w, b, acc.w));
+          l = fmaf(ml[x].y, b, l);
+        }
+      }
+    }
+    if (half) {
+      half_o[row] = acc;
+      half_ml[row] = make_float2(m, l);
+    }
+    __syncthreads();
+    if (!half && row_token < tp.tile_tokens && t0 + row_token < c.y) {
+      const int64_t token = c.x + t0 + row_token;
+      const int head = c.z * p.group + row_head;
+      const int64_t orow = token * p.heads + head, lse_at = static_cast<int64_t>(head) * p.total_q + token;
+      const float2 ml = half_ml[row];
+      const float4 o = half_o[row];
+      float other = -INFINITY;
+      float4 e = make_float4(0.f, 0.f, 0.f, 0.f);
+      if (p.add_o != nullptr) {
+        other = __ldcg(p.add_lse + lse_at) * 1.4426950408889634f;
+        e = __ldcg(reinterpret_cast<const float4*>(p.add_o + orow * 128) + col);
+      }
+      const float top = fmax3(m, ml.x, other);
+      if (top != -INFINITY) {
+        const float a = exp2f(m - top), b = exp2f(ml.x - top), x = exp2f(other - top);
+        l = l * a + ml.y * b + x;
+        acc = make_float4(acc.x * a + o.x * b + e.x * x, acc.y * a + o.y * b + e.y * x, acc.z * a + o.z * b + e.z * x,
+                          acc.w * a + o.w * b + e.w * x);
+        m = top;
+      }
+      const float inv = l == 0.f ? 0.f : 1.f / l;
+      acc = make_float4(acc.x * inv, acc.y * inv, acc.z * inv, acc.w * inv);
+      if (p.o != nullptr)
+        *reinterpret_cast<uint2*>(p.o + orow * 128 + col * 4) = make_uint2(pack_bf16x2(acc.x, acc.y), pack_bf16x2(acc.z, acc.w));
+      else
+        reinterpret_cast<float4*>(p.o32 + orow * 128)[col] = acc;
+      if (p.lse != nullptr && col == 0) p.lse[lse_at] = l == 0.f ? -INFINITY : m * kLn2 + logf(l);
+    }
+    __syncthreads();
+  }
+}
+
+}  // namespace fav4

@@ -39,4 +39,19 @@ inline bool encode_bshd(CUtensorMap* map, const void* base, int b, int s, int h,
             CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
 }
 
+// A bf16 tensor of `rank` dimensions (innermost first, 128 contiguous elements) whose outer strides are
+// given in elements; boxes of 64 elements x box[1..], 128-byte swizzle, zeros outside the tensor.
+inline bool encode_rows(CUtensorMap* map, const void* base, int rank, const cuuint64_t* dims, const long long* strides,
+                        const cuuint32_t* box) {
+  auto fn = encode_fn();
+  if (!fn) return false;
+  cuuint64_t bytes[4];
+  for (int i = 1; i < rank; ++i)  // the stride of a single entry is never used, but has to be valid
+    bytes[i - 1] = dims[i] > 1 ? static_cast<cuuint64_t>(strides[i]) * 2 : 256;
+  const cuuint32_t elem[5] = {1, 1, 1, 1, 1};
+  return fn(map, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, static_cast<cuuint32_t>(rank), const_cast<void*>(base), dims, bytes,
+            box, elem, CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+            CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
+}
+
 }  // namespace fav4
