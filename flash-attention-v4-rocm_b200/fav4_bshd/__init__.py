@@ -413,108 +413,6 @@ class Runner:
         if status:
             raise RuntimeError(f"backward: CUDA status {status}")
 
-    @staticmethod
-    def _row_strides(x):
-        ts, hs, ds = x.stride()
-        assert ds == 1
-        return ts if x.shape[0] > 1 else 0, hs if x.shape[1] > 1 else 0
-
-    def _paged_cache(self, k_cache, v_cache, page_table, seq_lens, device):
-        import torch
-        assert k_cache.dtype == v_cache.dtype == torch.bfloat16 and k_cache.device == v_cache.device == device
-        pages, size, hk, d = shape = k_cache.shape
-        ps, ts, hs, ds = strides = k_cache.stride()
-        assert d == HEAD_DIM and ds == 1 and v_cache.shape == shape and v_cache.stride() == strides
-        ps, hs = ps if pages > 1 else 0, hs if hk > 1 else 0  # the stride of a single entry says nothing
-        assert page_table.dtype == seq_lens.dtype == torch.int32 and page_table.device == seq_lens.device == device
-        batch, width = page_table.shape
-        assert seq_lens.shape == (batch,) and seq_lens.is_contiguous() and page_table.stride(1) == 1
-        return PagedCache(k_cache.data_ptr(), v_cache.data_ptr(), page_table.data_ptr(), seq_lens.data_ptr(), ps, ts,
-                          hs, page_table.stride(0), batch, hk, pages, size, width)
-
-    def _paged_workspace(self, a, device, stream):
-        """A workspace for each device and stream that calls (so calls on two streams may overlap), its
-        counters zeroed when it is made, and kept."""
-        import torch
-        need = self.lib.fav4_bshd_paged_workspace_bytes(C.byref(a))
-        if need == 0:
-            raise RuntimeError("paged attention: invalid arguments")
-        held = self.__dict__.setdefault("_paged_ws", {})
-        ws = held.get((device, stream))
-        if ws is None or ws.numel() < need:
-            ws = held[device, stream] = torch.empty(need, dtype=torch.uint8, device=device)
-            ws[:4096].zero_()  # the counters
-            current = torch.cuda.current_stream(device)
-            if current.cuda_stream != stream:
-                current.synchronize()  # the zeros are written on the current stream
-        return ws
-
-    def paged_append(self, q, k, v, q_out, k_cache, v_cache, page_table, seq_lens, cu_q, cos=None, sin=None,
-                     interleaved=False, offsets=None, stream=None):
-        """New keys and values into the pages, queries and keys rotated on the way (fav4_bshd_paged_append). q [T,
-        H, 128], k and v [T, H_kv, 128] may be strided (e.g. slices of one projection); q_out is contiguous; caches
-        [pages, page_size, H_kv, 128] (any strides, elements contiguous); page_table int32 [B, max_pages]; seq_lens
-        int32 [B], these tokens included; cu_q int32 [B + 1]; cos, sin FP32 [positions, rotary/2], or None for no
-        rotation; offsets: optional int32 [B] added to the rotation's positions."""
-        import torch
-        tokens, h, d = q.shape
-        assert q.dtype == k.dtype == v.dtype == q_out.dtype == torch.bfloat16 and d == HEAD_DIM and q.is_cuda
-        device = q.device
-        cache = self._paged_cache(k_cache, v_cache, page_table, seq_lens, device)
-        assert k.shape == v.shape == (tokens, cache.kv_heads, d) and q_out.shape == q.shape and q_out.is_contiguous()
-        assert k.device == v.device == q_out.device == cu_q.device == device
-        (qt, qh), (kt, kh), (vt, vh) = self._row_strides(q), self._row_strides(k), self._row_strides(v)
-        assert cu_q.dtype == torch.int32 and cu_q.shape == (cache.batch + 1,) and cu_q.is_contiguous()
-        rotary, rows = 0, 0
-        if cos is not None:
-            rows, half = cos.shape
-            rotary = 2 * half
-            assert cos.dtype == sin.dtype == torch.float32 and sin.shape == cos.shape and cos.is_contiguous()
-            assert sin.is_contiguous() and cos.device == sin.device == device
-        if offsets is not None:
-            assert offsets.dtype == torch.int32 and offsets.shape == (cache.batch,) and offsets.is_contiguous()
-            assert offsets.device == device
-        a = PagedAppendArgs(cache, q.data_ptr(), k.data_ptr(), v.data_ptr(), q_out.data_ptr(), cu_q.data_ptr(),
-                            _ptr(cos), _ptr(sin), _ptr(offsets), qt, qh, kt, kh, vt, vh, h, tokens, rotary,
-                            int(interleaved), rows)
-        status = self.lib.fav4_bshd_paged_append(C.byref(a), _stream(stream))
-        if status:
-            raise RuntimeError(f"paged_append: CUDA status {status}")
-
-    def call_paged(self, q, o, lse, k_cache, v_cache, page_table, seq_lens, cu_q, max_sq, causal=True, scale=None,
-                   prefix_pages=None, prefix_len=None, stream=None, workspace=None):
-        """Attention over the pages (fav4_bshd_forward_paged, or fav4_bshd_forward_shared_prefix when prefix_pages,
-        int32 [n], and prefix_len, int32 [1], name keys that stand before every sequence). q [T, H, 128], strided;
-        o [T, H, 128] contiguous; lse optional FP32 [H, T]; max_sq bounds the tokens of a sequence; the cache as in
-        paged_append. Causal is bottom-right: a sequence's rows are its newest keys. The workspace is allocated with
-        torch, one for each stream, and kept, unless one is given (its first 4096 bytes zero
-        before its first use)."""
-        import torch
-        tokens, h, d = q.shape
-        assert q.dtype == o.dtype == torch.bfloat16 and d == HEAD_DIM and q.is_cuda
-        device = q.device
-        cache = self._paged_cache(k_cache, v_cache, page_table, seq_lens, device)
-        qt, qh = self._row_strides(q)
-        assert o.shape == q.shape and o.is_contiguous() and o.device == cu_q.device == device
-        assert lse is None or (lse.shape == (h, tokens) and lse.dtype == torch.float32 and lse.is_contiguous()
-                               and lse.device == device)
-        assert cu_q.dtype == torch.int32 and cu_q.shape == (cache.batch + 1,) and cu_q.is_contiguous()
-        width = 0
-        if prefix_pages is not None:
-            assert prefix_pages.dtype == prefix_len.dtype == torch.int32 and prefix_pages.dim() == 1
-            assert prefix_pages.device == prefix_len.device == device and prefix_len.numel() == 1
-            assert prefix_pages.is_contiguous()
-            width = prefix_pages.shape[0]
-        a = PagedArgs(cache, q.data_ptr(), o.data_ptr(), _ptr(lse), cu_q.data_ptr(), _ptr(prefix_pages),
-                      _ptr(prefix_len), qt, qh, h, min(max_sq, tokens), tokens, width,
-                      1 / math.sqrt(HEAD_DIM) if scale is None else scale)
-        stream = _stream(stream)
-        ws = self._paged_workspace(a, device, stream) if workspace is None else workspace
-        entry = self.lib.fav4_bshd_forward_paged if width == 0 else self.lib.fav4_bshd_forward_shared_prefix
-        status = entry(C.byref(a), int(causal), ws.data_ptr(), ws.numel(), stream)
-        if status:
-            raise RuntimeError(f"paged attention: CUDA status {status}")
-
     def select_config(self, q, k, v, o, lse=None):
         a = self.args(q, k, v, o, lse)
         return self.lib.fav4_bshd_select_config(C.byref(a))

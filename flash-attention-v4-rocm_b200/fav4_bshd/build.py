@@ -6,7 +6,9 @@ Compiles csrc/fav4_bshd.cu and csrc/paged.cu -> build/libfav4_bshd.so (the C
 ABI of include/fav4_bshd.h) and csrc/probe.cu -> build/libfav4_probe.so (test probes)
 with nvcc for sm_100a, statically linked against the CUDA runtime. The ptxas
 resource report (registers, spills, shared memory) of each build is written
-next to the library as build/<lib>.ptxas.txt.
+next to the library as build/<lib>.ptxas.txt. csrc/paged_torch.cpp ->
+build/fav4_paged_torch.so is the PyTorch binding of the paged cache entries
+(host code only; it calls libfav4_bshd.so, which it finds beside itself).
 """
 from __future__ import annotations
 
@@ -29,6 +31,8 @@ TARGETS = {
     "libfav4_bshd.so": ["fav4_bshd.cu", "paged.cu"],
     "libfav4_probe.so": ["probe.cu"],
 }
+BINDING = "fav4_paged_torch.so"
+BINDING_SRC = CSRC / "paged_torch.cpp"
 
 
 def nvcc() -> str:
@@ -45,6 +49,33 @@ def _stale(out: Path, deps) -> bool:
     return any(d.stat().st_mtime > t for d in deps)
 
 
+def _run(cmd, log: Path, name: str, verbose: bool) -> None:
+    r = subprocess.run(cmd, capture_output=True, text=True)
+    log.write_text(r.stdout + r.stderr)
+    if r.returncode != 0:
+        sys.stderr.write(r.stdout + r.stderr)
+        raise RuntimeError(f"the compiler failed for {name}")
+    if verbose:
+        print(" ".join(cmd))
+
+
+def binding_command(out: Path) -> list[str]:
+    import sysconfig
+
+    import torch
+    from torch.utils import cpp_extension
+
+    home = Path(nvcc()).resolve().parents[1]
+    includes = [*cpp_extension.include_paths(), str(home / "include"), sysconfig.get_paths()["include"], str(INCLUDE)]
+    libs = Path(torch.__file__).parent / "lib"
+    cxx = os.environ.get("CXX") or shutil.which("g++") or "c++"
+    # the C++ runtime that torch itself runs on, never a static copy of the compiler's
+    return [cxx, "-O2", "-std=c++17", "-fPIC", "-shared", "-nostdlib++", f"-D_GLIBCXX_USE_CXX11_ABI={int(torch.compiled_with_cxx11_abi())}",
+            *[f"-isystem{i}" for i in includes], str(BINDING_SRC), "-o", str(out), f"-L{BUILD}", f"-L{libs}",
+            "-l:libfav4_bshd.so", "-lc10", "-lc10_cuda", "-ltorch_cpu", "-ltorch_python",
+            f"-L{home / 'lib64'}", "-lcudart", "-l:libstdc++.so.6", "-Wl,-rpath,$ORIGIN", f"-Wl,-rpath,{libs}"]
+
+
 def build(force: bool = False, verbose: bool = False) -> list[Path]:
     BUILD.mkdir(parents=True, exist_ok=True)
     deps = list(CSRC.glob("*.cu")) + list(CSRC.glob("*.cuh")) + list(CSRC.glob("*.h")) + list(INCLUDE.glob("*.h"))
@@ -53,15 +84,12 @@ def build(force: bool = False, verbose: bool = False) -> list[Path]:
         out = BUILD / lib
         if force or _stale(out, deps):
             cmd = [nvcc(), *ARCH_FLAGS, *COMMON, "-o", str(out), *[str(CSRC / s) for s in srcs]]
-            r = subprocess.run(cmd, capture_output=True, text=True)
-            (BUILD / f"{lib}.ptxas.txt").write_text(r.stdout + r.stderr)
-            if r.returncode != 0:
-                sys.stderr.write(r.stdout + r.stderr)
-                raise RuntimeError(f"nvcc failed for {lib}")
-            if verbose:
-                print(" ".join(cmd))
+            _run(cmd, BUILD / f"{lib}.ptxas.txt", lib, verbose)
         built.append(out)
-    return built
+    out = BUILD / BINDING
+    if force or _stale(out, [BINDING_SRC, *INCLUDE.glob("*.h")]):
+        _run(binding_command(out), BUILD / f"{BINDING}.log", BINDING, verbose)
+    return [*built, out]
 
 
 def main():
