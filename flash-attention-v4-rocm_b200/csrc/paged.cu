@@ -174,7 +174,7 @@ int launch_tiles(const PagedParams& p, const PagedSpace& sp, uint8_t* ws, int sm
   if (cudaError_t e = cudaGetLastError(); e != cudaSuccess) return e;
   // the join goes out as a programmatic dependent launch: it waits for the pieces itself
   cudaLaunchConfig_t cfg = {};
-  cfg.gridDim = dim3(2 * sms);
+  cfg.gridDim = dim3(kJoinPerSm * sms);
   cfg.blockDim = dim3(256);
   cfg.stream = stream;
   cudaLaunchAttribute attr[1];

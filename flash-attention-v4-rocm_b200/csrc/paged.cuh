@@ -27,6 +27,13 @@ struct SeqView {
   int q0, sq, len;
 };
 
+// a / b for a >= 0, b > 0. Work counts are 64-bit, but nearly always small: a 64-bit division costs several
+// times a 32-bit one, and the schedules wait for theirs.
+__host__ __device__ __forceinline__ int64_t quotient(int64_t a, int64_t b) {
+  if (((a | b) >> 32) == 0) return static_cast<uint32_t>(a) / static_cast<uint32_t>(b);
+  return a / b;
+}
+
 __device__ __forceinline__ SeqView seq_view(const PagedCacheView& c, const int* cu, int total_q, int max_sq, int b) {
   SeqView s;
   if (cu != nullptr) {
@@ -197,10 +204,11 @@ __global__ void __launch_bounds__(256) paged_append_kernel(const __grid_constant
 // tile; a unit that a boundary cuts leaves its pieces in the workspace, and the block that finishes
 // last joins them in the order of their keys (the sum does not depend on who that is).
 //
-// Inside a block the four warps never wait on one another: each takes every fourth 16-key group with
-// its own ring of asynchronous copies, its own m, l and O (16 x 128 in registers, mma.sync m16n8k16),
-// and they are joined once per piece. 16 rows keep the legacy tensor path busy well below its rate at
-// HBM speed: 64 instructions of 4096 multiply-adds for each 8 KiB.
+// Inside a block the four warps never wait on one another within a piece: each takes every fourth 16-key
+// group with its own ring of asynchronous copies, its own m, l and O (16 x 128 in registers, mma.sync
+// m16n8k16), and they are joined at the end of the piece, through the ring slots that they have just
+// used, while the copies of the next piece are under way. 16 rows keep the legacy tensor path busy well
+// below its rate at HBM speed: 64 instructions of 2048 multiply-adds for each 8 KiB.
 // ------------------------------------------------------------------------------------------------
 struct PagedParams {
   PagedCacheView c;
@@ -226,9 +234,9 @@ constexpr int kPagedWarps = 4;
 constexpr int kPagedStages = 3;
 constexpr int kPagedStageBytes = 2 * 16 * 256;  // 16 keys and 16 values
 constexpr int kPagedRing = kPagedStages * kPagedStageBytes;
-constexpr int kPagedPitch = 136;  // floats per row of the joining buffer: 8 rows x 2 floats on 32 banks
+constexpr int kPagedList = 64;   // pieces that are listed at a time
 constexpr int kPagedSmem = kPagedWarps * kPagedRing;
-static_assert(kPagedRows * kPagedPitch * 4 <= kPagedRing, "the joining buffer overlays the ring");
+static_assert(kPagedRows * 128 * 4 <= kPagedStageBytes, "a warp's O is left in one ring slot");
 
 __device__ __forceinline__ void cp_async16(uint32_t dst, const void* src, int bytes) {
   asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(bytes) : "memory");
@@ -274,7 +282,7 @@ struct RowPlace {
 };
 __device__ __forceinline__ bool row_place(const PagedParams& p, const SeqView& s, int h, int64_t r, RowPlace* out) {
   if (r >= static_cast<int64_t>(s.sq) * p.group) return false;
-  const int i = static_cast<int>(r / p.group);
+  const int i = static_cast<int>(quotient(r, p.group));
   out->token = s.q0 + i;
   out->head = h * p.group + static_cast<int>(r - static_cast<int64_t>(i) * p.group);
   return true;
@@ -307,309 +315,415 @@ __device__ __forceinline__ void finish_row(const PagedParams& p, const RowPlace&
   if (p.lse != nullptr && lane == 0) p.lse[lse_at] = l == 0.f ? -INFINITY : m * 0.6931471805599453f + logf(l);
 }
 
+// A stretch of one unit, as this block takes it.
+struct PagedPiece {
+  int b, h, r0, sq;               // sequence, K/V head, first row, tokens
+  int q0, len, key_begin, groups; // first packed row, keys; the piece's first key and its 16-key groups
+  int tile0, cnt, n, c0;          // tiles [tile0, tile0 + cnt) of n; blocks c0..c1 hold the unit
+  int c1, pad[3];
+};
+static_assert(sizeof(PagedPiece) == 64, "four 16-byte words");
+
+// Inclusive sum over the block's threads; *sum is the total. Ends with every thread past its reads of `tmp`.
+template <typename T>
+__device__ __forceinline__ T block_scan(T v, T* tmp, T* sum) {
+  const int warp = threadIdx.x / 32, lane = threadIdx.x % 32;
+#pragma unroll
+  for (int o = 1; o < 32; o *= 2) {
+    const T up = __shfl_up_sync(0xffffffffu, v, o);
+    if (lane >= o) v += up;
+  }
+  if (lane == 31) tmp[warp] = v;
+  __syncthreads();
+  T all = 0;
+#pragma unroll
+  for (int w = 0; w < kPagedWarps; ++w) {
+    if (w < warp) v += tmp[w];
+    all += tmp[w];
+  }
+  *sum = all;
+  __syncthreads();
+  return v;
+}
+
+// Byte offset of 4-column piece c of row r of a 16 x 128 FP32 tile in a ring slot, spread over the banks.
+__device__ __forceinline__ int tile_at(int r, int c) { return r * 512 + ((c ^ (r & 7)) * 16); }
+
 __global__ void __launch_bounds__(kPagedWarps * 32, 2) paged_attn_kernel(const __grid_constant__ PagedParams p) {
   extern __shared__ __align__(1024) uint8_t smem[];
-  __shared__ int64_t scan[kPagedWarps];
-  __shared__ int64_t found_base;
-  __shared__ int found_seq;
+  __shared__ __align__(16) PagedPiece list[kPagedList];
+  __shared__ int64_t scan64[kPagedWarps];
+  __shared__ int scan32[kPagedWarps];
   __shared__ float piece_ml[kPagedWarps][kPagedRows][2];
+  __shared__ int free_slot[kPagedWarps];
   __shared__ uint32_t last_one;
   const int tid = threadIdx.x, warp = tid / 32, lane = tid % 32;
-
-  // ---- this block's stretch [begin, end) of the line of tiles, and the sequence it begins in ----
-  int64_t total = 0, begin = 0, per = 0;
-  for (int pass = 0; pass < 2; ++pass) {
-    int64_t base = 0;
-    for (int b0 = 0; b0 < p.c.batch; b0 += kPagedWarps * 32) {
-      const int b = b0 + tid;
-      int64_t v = b < p.c.batch ? paged_seq_work(p, seq_view(p.c, p.cu, p.total_q, p.max_sq, b)) : 0;
-      const int64_t mine = v;
-#pragma unroll
-      for (int o = 1; o < 32; o *= 2) {
-        const int64_t up = __shfl_up_sync(0xffffffffu, v, o);
-        if (lane >= o) v += up;
-      }
-      if (lane == 31) scan[warp] = v;
-      __syncthreads();
-      int64_t sum = 0;
-#pragma unroll
-      for (int w = 0; w < kPagedWarps; ++w) {
-        if (w < warp) v += scan[w];
-        sum += scan[w];
-      }
-      if (p.c.batch <= kPagedWarps * 32) {  // one step sees the whole batch: no second pass
-        total = sum;
-        per = (total + gridDim.x - 1) / gridDim.x;
-        begin = blockIdx.x * per;
-        pass = 1;
-      }
-      if (pass == 1 && base + v - mine <= begin && begin < base + v) {
-        found_seq = b;
-        found_base = base + v - mine;
-      }
-      base += sum;
-      __syncthreads();
-    }
-    if (pass == 0) {
-      total = base;
-      per = (total + gridDim.x - 1) / gridDim.x;
-      begin = blockIdx.x * per;
-    }
-  }
-  const int64_t end = min(total, begin + per);
-  if (begin >= end) return;
-  int b = found_seq;
-  int64_t base = found_base;
-
+  const int g = lane / 4, t4 = lane % 4;     // mma fragments: rows g and g + 8, columns 2 t4 and 2 t4 + 1 of eight
+  const int mi = lane / 8, mr = lane % 8;    // ldmatrix: matrix and row that this lane addresses
+  const int cl = lane % 16, rl = lane / 16;  // copies: 16-byte piece cl of rows rl + 2 j
   const uint32_t ring = smem_addr(smem) + warp * kPagedRing;
-  float* join = reinterpret_cast<float*>(smem + warp * kPagedRing);
 
-  for (int64_t pos = begin; pos < end;) {
-    const SeqView s = seq_view(p.c, p.cu, p.total_q, p.max_sq, b);
-    const int64_t work = paged_seq_work(p, s);
-    if (pos >= base + work) {  // this sequence is done
-      base += work;
-      ++b;
-      continue;
+  int64_t total = 0, per = 0, begin = 0, end = 0;
+  for (int round = 0;; ++round) {
+    // ---- the pieces of this block's stretch [begin, end) of the line of tiles, kPagedList at a time ----
+    int pieces = 0;  // of the whole stretch
+    for (int pass = round == 0 ? 0 : 1; pass < 2; ++pass) {
+      int64_t base = 0;
+      pieces = 0;
+      for (int b0 = 0; b0 < p.c.batch; b0 += kPagedWarps * 32) {
+        const int b = b0 + tid;
+        SeqView s = {0, 0, 0};
+        if (b < p.c.batch) s = seq_view(p.c, p.cu, p.total_q, p.max_sq, b);
+        const int64_t work = paged_seq_work(p, s);
+        int64_t sum;
+        const int64_t first_tile = base + block_scan(work, scan64, &sum) - work;  // of this sequence
+        if (p.c.batch <= kPagedWarps * 32) pass = 1;  // one step sees the whole batch
+        if (round == 0 && p.c.batch <= kPagedWarps * 32) {
+          total = sum;
+          per = quotient(total + gridDim.x - 1, gridDim.x);
+          begin = blockIdx.x * per;
+          end = min(total, begin + per);
+        }
+        if (pass == 1) {
+          const int64_t lo = max(begin, first_tile), hi = min(end, first_tile + work);
+          const int n = paged_tiles(s);
+          int mine = 0;
+          int64_t u = 0;
+          if (lo < hi) {
+            u = quotient(lo - first_tile, n);
+            mine = static_cast<int>(quotient(hi - 1 - first_tile, n) - u) + 1;
+          }
+          int listed;
+          int at = pieces + block_scan(mine, scan32, &listed) - mine - round * kPagedList;
+          pieces += listed;
+          const int64_t rows = static_cast<int64_t>(s.sq) * p.group;
+          const int64_t blocks = (rows + kPagedRows - 1) / kPagedRows;
+          for (; mine > 0; --mine, ++u, ++at) {
+            if (at < 0 || at >= kPagedList) continue;
+            PagedPiece w;
+            w.b = b;
+            w.h = static_cast<int>(quotient(u, blocks));
+            w.r0 = static_cast<int>(u - w.h * blocks) * kPagedRows;
+            w.sq = s.sq;
+            w.q0 = s.q0;
+            w.len = s.len;
+            const int64_t first = first_tile + u * n;  // the unit's place on the line
+            w.tile0 = static_cast<int>(max(begin - first, int64_t(0)));
+            w.cnt = static_cast<int>(min(static_cast<int64_t>(n), end - first)) - w.tile0;
+            w.n = n;
+            w.c0 = static_cast<int>(quotient(first, per));
+            w.c1 = static_cast<int>(quotient(first + n - 1, per));
+            w.key_begin = w.tile0 * kPagedTile;
+            int64_t key_end = min((w.tile0 + static_cast<int64_t>(w.cnt)) * kPagedTile, static_cast<int64_t>(s.len));
+            if (p.causal)  // the last key that the block's last row sees
+              key_end = min(key_end, static_cast<int64_t>(s.len) - s.sq + 1 +
+                                         quotient(min(static_cast<int64_t>(w.r0) + kPagedRows, rows) - 1, p.group));
+            w.groups = static_cast<int>(max(key_end - w.key_begin + 15, int64_t(0)) / 16);
+            list[at] = w;
+          }
+        }
+        base += sum;
+      }
+      if (pass == 0) {
+        total = base;
+        per = quotient(total + gridDim.x - 1, gridDim.x);
+        begin = blockIdx.x * per;
+        end = min(total, begin + per);
+      }
     }
-    const int n = paged_tiles(s);
-    const int blocks = static_cast<int>((static_cast<int64_t>(s.sq) * p.group + kPagedRows - 1) / kPagedRows);
-    const int64_t unit = (pos - base) / n;
-    const int tile0 = static_cast<int>(pos - base - unit * n);
-    const int cnt = static_cast<int>(min(static_cast<int64_t>(n - tile0), end - pos));
-    const int h = static_cast<int>(unit / blocks);
-    const int64_t r0 = (unit - static_cast<int64_t>(h) * blocks) * kPagedRows;
+    const int count = min(pieces - round * kPagedList, kPagedList);
+    if (count <= 0) return;
+    __syncthreads();
 
-    // last visible key of this thread's rows (g and g + 8), and of the whole row block
-    const int g = lane / 4, t4 = lane % 4;
-    const int64_t rows = static_cast<int64_t>(s.sq) * p.group;
-    const int past = s.len - s.sq;
-    int lim[2];
-#pragma unroll
-    for (int u = 0; u < 2; ++u) {
-      const int64_t r = min(r0 + g + 8 * u, rows - 1);
-      lim[u] = p.causal ? past + static_cast<int>(r / p.group) : s.len - 1;
-    }
-    const int lim_max =
-        p.causal ? past + static_cast<int>(min(r0 + kPagedRows - 1, rows - 1) / p.group) : s.len - 1;
-    const int lim_min = p.causal ? past + static_cast<int>(r0 / p.group) : s.len - 1;
-    const int key_begin = tile0 * kPagedTile;
-    const int64_t key_stop = static_cast<int64_t>(tile0 + cnt) * kPagedTile;
-    const int key_end = static_cast<int>(min(key_stop, static_cast<int64_t>(min(s.len, lim_max + 1))));
-    const int groups = max(key_end - key_begin + 15, 0) / 16;
-    const int steps = (groups - warp + kPagedWarps - 1) / kPagedWarps;  // this warp's 16-key groups (<= 0: none)
-
-    // ring: lane copies piece lane % 16 of rows lane / 16 + 2 j
-    const int64_t head_off = h * p.c.head_stride;
-    const int* table = p.c.table + b * p.c.table_stride;
-    const int cl = lane % 16, rl = lane / 16;
-    auto key_of = [&](int i) { return key_begin + (warp + kPagedWarps * i) * 16; };
-    auto page_of = [&](int i) { return i < steps ? __ldg(table + key_of(i) / p.c.page_size) : 0; };
-    auto issue = [&](int i, int page) {
-      if (i < steps) {
-        const int key = key_of(i);
-        page = min(max(page, 0), p.c.num_pages - 1);
-        const int64_t off = page * p.c.page_stride + (key % p.c.page_size + rl) * p.c.token_stride + head_off + cl * 8;
+    // ---- copies: this warp's 16-key groups of all listed pieces, kPagedStages - 1 ahead of their use ----
+    // A stretch of up to 32 groups of a piece has its page numbers in the lanes; those of the stretch after it
+    // are loaded when it begins.
+    auto steps_of = [&](int i) { return (list[i].groups - warp + kPagedWarps - 1) / kPagedWarps; };
+    auto pages_from = [&](int i, int s0) -> int {
+      if (i >= count || s0 + lane >= steps_of(i)) return 0;
+      const int key = list[i].key_begin + (warp + kPagedWarps * (s0 + lane)) * 16;
+      const int page = __ldg(p.c.table + list[i].b * p.c.table_stride + key / p.c.page_size);
+      return min(max(page, 0), p.c.num_pages - 1);
+    };
+    auto skip_empty = [&](int i) {
+      while (i < count && steps_of(i) <= 0) ++i;
+      return i;
+    };
+    int li = skip_empty(0), ls = 0;  // next group to copy: step ls of piece li
+    int l_stop = 0, l_key = 0, l_len = 0, n_piece = 0, n_from = 0;
+    int64_t l_head = 0;
+    int pages = pages_from(li, 0), pages_next = 0;
+    auto open = [&]() {  // the stretch that holds step ls of piece li begins; the one after it is looked up
+      if (li >= count) return;
+      const int steps = steps_of(li);
+      l_stop = min(steps, ls + 32);
+      l_key = list[li].key_begin + warp * 16;
+      l_len = list[li].len;
+      l_head = list[li].h * p.c.head_stride + cl * 8;
+      n_piece = l_stop < steps ? li : skip_empty(li + 1);
+      n_from = l_stop < steps ? l_stop : 0;
+      pages_next = pages_from(n_piece, n_from);
+    };
+    open();
+    int slot_in = 0;  // ring slot of the next copy
+    auto issue = [&]() {
+      if (li < count) {
+        const int key = l_key + ls * (kPagedWarps * 16);
+        const int64_t page = __shfl_sync(0xffffffffu, pages, ls % 32);
+        const int64_t off = page * p.c.page_stride + (key % p.c.page_size + rl) * p.c.token_stride + l_head;
         const __nv_bfloat16* ks = p.c.k + off;
         const __nv_bfloat16* vs = p.c.v + off;
-        const uint32_t dst = ring + (i % kPagedStages) * kPagedStageBytes + rl * 256;
+        const uint32_t dst = ring + slot_in * kPagedStageBytes + rl * 256;
 #pragma unroll
         for (int j = 0; j < 8; ++j) {
           const int row = rl + 2 * j;
-          const int bytes = key + row < s.len ? 16 : 0;  // slots past the end may hold anything: zeros instead
+          const int bytes = key + row < l_len ? 16 : 0;  // slots past the end may hold anything: zeros instead
           const uint32_t d = dst + j * 512 + ((cl ^ (row & 7)) * 16);
           cp_async16(d, ks + 2 * j * p.c.token_stride, bytes);
           cp_async16(d + 4096, vs + 2 * j * p.c.token_stride, bytes);
         }
+        if (++ls == l_stop) {
+          li = n_piece;
+          ls = n_from;
+          pages = pages_next;
+          open();
+        }
       }
       cp_async_commit();
+      slot_in = slot_in == kPagedStages - 1 ? 0 : slot_in + 1;
     };
-    int page_next = page_of(0);
 #pragma unroll
-    for (int i = 0; i < kPagedStages - 1; ++i) {
-      const int page = page_next;
-      page_next = page_of(i + 1);
-      issue(i, page);
-    }
-    uint32_t qf[8][4];
-#pragma unroll
-    for (int u = 0; u < 2; ++u) {
-      RowPlace at;
-      const bool live = row_place(p, s, h, r0 + g + 8 * u, &at);
-      const __nv_bfloat16* src = live ? p.q + at.token * p.q_ts + at.head * p.q_hs + t4 * 2 : nullptr;
-#pragma unroll
-      for (int k = 0; k < 8; ++k) {
-        qf[k][u] = live ? __ldg(reinterpret_cast<const uint32_t*>(src + k * 16)) : 0u;
-        qf[k][u + 2] = live ? __ldg(reinterpret_cast<const uint32_t*>(src + k * 16 + 8)) : 0u;
-      }
-    }
+    for (int i = 0; i < kPagedStages - 1; ++i) issue();
 
-    float o[16][4];
-#pragma unroll
-    for (int j = 0; j < 16; ++j) o[j][0] = o[j][1] = o[j][2] = o[j][3] = 0.f;
-    float m[2] = {-INFINITY, -INFINITY}, l[2] = {0.f, 0.f};
-    const int mi = lane / 8, mr = lane % 8;
-    for (int i = 0; i < steps; ++i) {
-      cp_async_wait<kPagedStages - 2>();
-      __syncwarp();  // group i has arrived, and every lane is done with group i - 1
-      const int page = page_next;
-      page_next = page_of(i + kPagedStages);
-      issue(i + kPagedStages - 1, page);
-      const uint32_t st = ring + (i % kPagedStages) * kPagedStageBytes;
-      float sc[2][4] = {};
-#pragma unroll
-      for (int k = 0; k < 8; ++k) {
-        uint32_t kb[4];
-        ldsm4(st + ((mi / 2) * 8 + mr) * 256 + (((2 * k + (mi & 1)) ^ mr) * 16), kb);
-        mma16816(sc[0], qf[k], kb[0], kb[1]);
-        mma16816(sc[1], qf[k], kb[2], kb[3]);
-      }
-      const int key = key_of(i);
-      if (key + 15 > lim_min) {
-#pragma unroll
-        for (int e = 0; e < 8; ++e) {
-          const int col = key + (e / 4) * 8 + t4 * 2 + (e & 1);
-          if (col > lim[(e / 2) & 1]) sc[e / 4][e % 4] = -INFINITY;
-        }
-      }
-      bool grow = false;
-      float cand[2];
+    uint32_t qf[8][4];
+    auto load_q = [&](int i) {
+      const PagedPiece& w = list[i];
 #pragma unroll
       for (int u = 0; u < 2; ++u) {
-        float mx = fmaxf(fmaxf(sc[0][2 * u], sc[0][2 * u + 1]), fmaxf(sc[1][2 * u], sc[1][2 * u + 1]));
-        mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 1));
-        mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 2));
-        cand[u] = fmaxf(m[u], mx * p.scale_log2);
-        grow |= cand[u] > m[u] + 8.f;  // the sums are rescaled only when a maximum grows by 2^8
+        const int r = w.r0 + g + 8 * u, token = r / p.group;
+        const bool live = token < w.sq;
+        const __nv_bfloat16* src =
+            p.q + (w.q0 + token) * p.q_ts + (w.h * p.group + r - token * p.group) * p.q_hs + t4 * 2;
+#pragma unroll
+        for (int k = 0; k < 8; ++k) {
+          qf[k][u] = live ? __ldg(reinterpret_cast<const uint32_t*>(src + k * 16)) : 0u;
+          qf[k][u + 2] = live ? __ldg(reinterpret_cast<const uint32_t*>(src + k * 16 + 8)) : 0u;
+        }
       }
-      if (__any_sync(0xffffffffu, grow)) {
+    };
+    load_q(0);
+
+    int slot = 0;  // ring slot of the next group to use
+    for (int i = 0; i < count; ++i) {
+      const int len = list[i].len, sq = list[i].sq, r0 = list[i].r0;
+      const int steps = steps_of(i);
+      // last visible key of this thread's rows (g and g + 8), and of the first row of all
+      int lim[2];
+#pragma unroll
+      for (int u = 0; u < 2; ++u)
+        lim[u] = p.causal ? len - sq + min((r0 + g + 8 * u) / p.group, sq - 1) : len - 1;
+      const int lim_min = p.causal ? len - sq + r0 / p.group : len - 1;
+      int key = list[i].key_begin + warp * 16;
+
+      float o[16][4];
+#pragma unroll
+      for (int j = 0; j < 16; ++j) o[j][0] = o[j][1] = o[j][2] = o[j][3] = 0.f;
+      float m[2] = {-INFINITY, -INFINITY}, l[2] = {0.f, 0.f};
+      for (int st_i = 0; st_i < steps; ++st_i, key += kPagedWarps * 16) {
+        cp_async_wait<kPagedStages - 2>();
+        __syncwarp();  // this group has arrived, and every lane is done with the one before
+        issue();
+        const uint32_t st = ring + slot * kPagedStageBytes;
+        slot = slot == kPagedStages - 1 ? 0 : slot + 1;
+        float sc[2][4] = {};
+#pragma unroll
+        for (int k = 0; k < 8; ++k) {
+          uint32_t kb[4];
+          ldsm4(st + ((mi / 2) * 8 + mr) * 256 + (((2 * k + (mi & 1)) ^ mr) * 16), kb);
+          mma16816(sc[0], qf[k], kb[0], kb[1]);
+          mma16816(sc[1], qf[k], kb[2], kb[3]);
+        }
+        if (key + 15 > lim_min) {
+#pragma unroll
+          for (int e = 0; e < 8; ++e) {
+            const int col = key + (e / 4) * 8 + t4 * 2 + (e & 1);
+            if (col > lim[(e / 2) & 1]) sc[e / 4][e % 4] = -INFINITY;
+          }
+        }
+        bool grow = false;
+        float cand[2];
 #pragma unroll
         for (int u = 0; u < 2; ++u) {
-          const float a = cand[u] == -INFINITY ? 1.f : ex2_mufu(m[u] - cand[u]);
-          m[u] = cand[u];
-          l[u] *= a;
+          float mx = fmaxf(fmaxf(sc[0][2 * u], sc[0][2 * u + 1]), fmaxf(sc[1][2 * u], sc[1][2 * u + 1]));
+          mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 1));
+          mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 2));
+          cand[u] = fmaxf(m[u], mx * p.scale_log2);
+          grow |= cand[u] > m[u] + 8.f;  // the sums are rescaled only when a maximum grows by 2^8
+        }
+        if (__any_sync(0xffffffffu, grow)) {
 #pragma unroll
-          for (int j = 0; j < 16; ++j) {
-            o[j][2 * u] *= a;
-            o[j][2 * u + 1] *= a;
+          for (int u = 0; u < 2; ++u) {
+            const float a = cand[u] == -INFINITY ? 1.f : ex2_mufu(m[u] - cand[u]);
+            m[u] = cand[u];
+            l[u] *= a;
+#pragma unroll
+            for (int j = 0; j < 16; ++j) {
+              o[j][2 * u] *= a;
+              o[j][2 * u + 1] *= a;
+            }
           }
         }
+        uint32_t pf[4];
+#pragma unroll
+        for (int u = 0; u < 2; ++u) {
+          const float mb = m[u] == -INFINITY ? 0.f : m[u];
+          const float p0 = ex2_mufu(fmaf(sc[0][2 * u], p.scale_log2, -mb));
+          const float p1 = ex2_mufu(fmaf(sc[0][2 * u + 1], p.scale_log2, -mb));
+          const float p2 = ex2_mufu(fmaf(sc[1][2 * u], p.scale_log2, -mb));
+          const float p3 = ex2_mufu(fmaf(sc[1][2 * u + 1], p.scale_log2, -mb));
+          l[u] += (p0 + p1) + (p2 + p3);
+          pf[u] = pack_bf16x2(p0, p1);  // P in BF16 for the second product; l sums the unrounded values
+          pf[u + 2] = pack_bf16x2(p2, p3);
+        }
+#pragma unroll
+        for (int j = 0; j < 8; ++j) {
+          uint32_t vb[4];
+          ldsm4_t(st + 4096 + ((mi & 1) * 8 + mr) * 256 + (((2 * j + mi / 2) ^ mr) * 16), vb);
+          mma16816(o[2 * j], pf, vb[0], vb[1]);
+          mma16816(o[2 * j + 1], pf, vb[2], vb[3]);
+        }
       }
-      uint32_t pf[4];
+      if (i + 1 < count) load_q(i + 1);  // arrives while this piece is joined
+
+      // ---- join the four warps: each leaves its O in the ring slot that no copy is under way to ----
+      const int spare = slot == 0 ? kPagedStages - 1 : slot - 1;
+      __syncwarp();
+      uint8_t* mine = smem + warp * kPagedRing + spare * kPagedStageBytes;
 #pragma unroll
       for (int u = 0; u < 2; ++u) {
-        const float mb = m[u] == -INFINITY ? 0.f : m[u];
-        const float p0 = ex2_mufu(fmaf(sc[0][2 * u], p.scale_log2, -mb));
-        const float p1 = ex2_mufu(fmaf(sc[0][2 * u + 1], p.scale_log2, -mb));
-        const float p2 = ex2_mufu(fmaf(sc[1][2 * u], p.scale_log2, -mb));
-        const float p3 = ex2_mufu(fmaf(sc[1][2 * u + 1], p.scale_log2, -mb));
-        l[u] += (p0 + p1) + (p2 + p3);
-        pf[u] = pack_bf16x2(p0, p1);  // P in BF16 for the second product; l sums the unrounded values
-        pf[u + 2] = pack_bf16x2(p2, p3);
-      }
+        l[u] += __shfl_xor_sync(0xffffffffu, l[u], 1);
+        l[u] += __shfl_xor_sync(0xffffffffu, l[u], 2);
+        if (t4 == 0) {
+          piece_ml[warp][g + 8 * u][0] = m[u];
+          piece_ml[warp][g + 8 * u][1] = l[u];
+        }
 #pragma unroll
-      for (int j = 0; j < 8; ++j) {
-        uint32_t vb[4];
-        ldsm4_t(st + 4096 + ((mi & 1) * 8 + mr) * 256 + (((2 * j + mi / 2) ^ mr) * 16), vb);
-        mma16816(o[2 * j], pf, vb[0], vb[1]);
-        mma16816(o[2 * j + 1], pf, vb[2], vb[3]);
+        for (int j = 0; j < 16; ++j)
+          *reinterpret_cast<float2*>(mine + tile_at(g + 8 * u, 2 * j + t4 / 2) + (t4 & 1) * 8) =
+              make_float2(o[j][2 * u], o[j][2 * u + 1]);
       }
-    }
-
-    // ---- join the four warps ----
-    cp_async_wait<0>();
-    __syncwarp();
-#pragma unroll
-    for (int u = 0; u < 2; ++u) {
-      l[u] += __shfl_xor_sync(0xffffffffu, l[u], 1);
-      l[u] += __shfl_xor_sync(0xffffffffu, l[u], 2);
-      if (t4 == 0) {
-        piece_ml[warp][g + 8 * u][0] = m[u];
-        piece_ml[warp][g + 8 * u][1] = l[u];
-      }
-#pragma unroll
-      for (int j = 0; j < 16; ++j)
-        *reinterpret_cast<float2*>(join + (g + 8 * u) * kPagedPitch + j * 8 + t4 * 2) =
-            make_float2(o[j][2 * u], o[j][2 * u + 1]);
-    }
-    __syncthreads();
-    const bool whole = cnt == n;
-    const int slot = 2 * blockIdx.x + (tile0 == 0 ? 1 : 0);  // a piece that opens its unit, or one that carries on
-    for (int r = warp; r < kPagedRows && r0 + r < rows; r += kPagedWarps) {
-      float top = piece_ml[0][r][0];
-#pragma unroll
-      for (int w = 1; w < kPagedWarps; ++w) top = fmaxf(top, piece_ml[w][r][0]);
-      float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
-      float sum = 0.f;
-#pragma unroll
-      for (int w = 0; w < kPagedWarps; ++w) {
-        const float mw = piece_ml[w][r][0];
-        const float a = mw == -INFINITY ? 0.f : exp2f(mw - top);
-        const float4 v =
-            *reinterpret_cast<const float4*>(reinterpret_cast<float*>(smem + w * kPagedRing) + r * kPagedPitch + lane * 4);
-        acc = make_float4(acc.x + a * v.x, acc.y + a * v.y, acc.z + a * v.z, acc.w + a * v.w);
-        sum += a * piece_ml[w][r][1];
-      }
-      if (whole) {
-        RowPlace at;
-        row_place(p, s, h, r0 + r, &at);
-        finish_row(p, at, acc, top, sum, lane);
-      } else {
-        *reinterpret_cast<float4*>(p.part_o + (static_cast<int64_t>(slot) * kPagedRows + r) * 128 + lane * 4) = acc;
-        if (lane == 0)
-          *reinterpret_cast<float2*>(p.part_ml + (static_cast<int64_t>(slot) * kPagedRows + r) * 2) =
-              make_float2(top, sum);
-      }
-    }
-    if (!whole) {
-      // the blocks of this unit: from the one that holds its first tile to the one that holds its last
-      const int64_t first_pos = pos - tile0;
-      const int c0 = static_cast<int>(first_pos / per), c1 = static_cast<int>((first_pos + n - 1) / per);
-      __threadfence();
+      if (lane == 0) free_slot[warp] = spare;
       __syncthreads();
-      if (tid == 0) {
-        const uint32_t before = atomicAdd(p.arrived + c0, 1u);
-        last_one = before == static_cast<uint32_t>(c1 - c0);
-        if (last_one) p.arrived[c0] = 0u;  // ready for the next launch
-      }
-      __syncthreads();
-      if (last_one) {
-        __threadfence();
-        for (int r = warp; r < kPagedRows && r0 + r < rows; r += kPagedWarps) {
-          auto slot_row = [&](int c) { return static_cast<int64_t>(2 * c + (c == c0 ? 1 : 0)) * kPagedRows + r; };
-          float top = -INFINITY;
-          for (int c = c0 + lane; c <= c1; c += 32) top = fmaxf(top, __ldcg(p.part_ml + slot_row(c) * 2));
+      const PagedPiece& w = list[i];
+      const int rows = static_cast<int>(min(static_cast<int64_t>(kPagedRows), static_cast<int64_t>(sq) * p.group - r0));
+      const bool whole = w.cnt == w.n;
+      const SeqView s = {w.q0, sq, len};
+      const int part = 2 * blockIdx.x + (w.tile0 == 0 ? 1 : 0);  // a piece that opens its unit, or one that carries on
+      for (int r = warp; r < rows; r += kPagedWarps) {
+        float top = piece_ml[0][r][0];
 #pragma unroll
-          for (int x = 16; x > 0; x /= 2) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, x));
-          float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
-          float sum = 0.f;
-          for (int c = c0; c <= c1; c += 8) {
-            float4 v[8];
-            float2 ml[8];
+        for (int x = 1; x < kPagedWarps; ++x) top = fmaxf(top, piece_ml[x][r][0]);
+        float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
+        float sum = 0.f;
 #pragma unroll
-            for (int x = 0; x < 8; ++x) {
-              if (c + x <= c1) {
-                v[x] = __ldcg(reinterpret_cast<const float4*>(p.part_o + slot_row(c + x) * 128 + lane * 4));
-                ml[x] = __ldcg(reinterpret_cast<const float2*>(p.part_ml + slot_row(c + x) * 2));
-              }
-            }
-#pragma unroll
-            for (int x = 0; x < 8; ++x) {
-              if (c + x <= c1 && ml[x].x != -INFINITY) {
-                const float a = exp2f(ml[x].x - top);
-                acc = make_float4(acc.x + a * v[x].x, acc.y + a * v[x].y, acc.z + a * v[x].z, acc.w + a * v[x].w);
-                sum += a * ml[x].y;
-              }
-            }
-          }
+        for (int x = 0; x < kPagedWarps; ++x) {
+          const float mx = piece_ml[x][r][0];
+          const float a = mx == -INFINITY ? 0.f : exp2f(mx - top);
+          const float4 v = *reinterpret_cast<const float4*>(smem + x * kPagedRing + free_slot[x] * kPagedStageBytes +
+                                                            tile_at(r, lane));
+          acc = make_float4(acc.x + a * v.x, acc.y + a * v.y, acc.z + a * v.z, acc.w + a * v.w);
+          sum += a * piece_ml[x][r][1];
+        }
+        if (whole) {
           RowPlace at;
-          row_place(p, s, h, r0 + r, &at);
+          row_place(p, s, w.h, r0 + r, &at);
           finish_row(p, at, acc, top, sum, lane);
+        } else {
+          *reinterpret_cast<float4*>(p.part_o + (static_cast<int64_t>(part) * kPagedRows + r) * 128 + lane * 4) = acc;
+          if (lane == 0)
+            *reinterpret_cast<float2*>(p.part_ml + (static_cast<int64_t>(part) * kPagedRows + r) * 2) =
+                make_float2(top, sum);
         }
       }
+      if (!whole) {
+        __threadfence();
+        __syncthreads();
+        if (tid == 0) {
+          const uint32_t before = atomicAdd(p.arrived + w.c0, 1u);
+          last_one = before == static_cast<uint32_t>(w.c1 - w.c0);
+          if (last_one) p.arrived[w.c0] = 0u;  // ready for the next launch
+        }
+        __syncthreads();
+        if (last_one) {
+          // this block is the last of the unit's: it adds the pieces up in the order of their keys. With fewer
+          // rows than warps, the warps share a row's pieces.
+          __threadfence();
+          const int share = rows == 1 ? 4 : rows == 2 ? 2 : 1;
+          const int turn = warp % share, parts = w.c1 - w.c0 + 1;
+          const int x_begin = parts * turn / share, x_end = parts * (turn + 1) / share;
+          for (int r = warp / share; r < rows; r += kPagedWarps / share) {
+            auto part_row = [&](int x) { return static_cast<int64_t>(2 * (w.c0 + x) + (x == 0 ? 1 : 0)) * kPagedRows + r; };
+            float top = -INFINITY, sum = 0.f;
+            float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
+            for (int x0 = x_begin; x0 < x_end; x0 += 12) {
+              float4 v[12];
+              float2 ml[12];
+#pragma unroll
+              for (int x = 0; x < 12; ++x) {
+                ml[x] = make_float2(-INFINITY, 0.f);
+                v[x] = make_float4(0.f, 0.f, 0.f, 0.f);
+                if (x0 + x < x_end) {
+                  v[x] = __ldcg(reinterpret_cast<const float4*>(p.part_o + part_row(x0 + x) * 128 + lane * 4));
+                  ml[x] = __ldcg(reinterpret_cast<const float2*>(p.part_ml + part_row(x0 + x) * 2));
+                }
+              }
+              float next = top;
+#pragma unroll
+              for (int x = 0; x < 12; ++x) next = fmaxf(next, ml[x].x);
+              // relative to 0 while no piece has seen a key: NaN sums still go through
+              const float zero = next == -INFINITY ? 0.f : next, a = exp2f(top - zero);
+              acc = make_float4(acc.x * a, acc.y * a, acc.z * a, acc.w * a);
+              sum *= a;
+              top = next;
+#pragma unroll
+              for (int x = 0; x < 12; ++x) {
+                const float c = exp2f(ml[x].x - zero);
+                acc = make_float4(acc.x + c * v[x].x, acc.y + c * v[x].y, acc.z + c * v[x].z, acc.w + c * v[x].w);
+                sum += c * ml[x].y;
+              }
+            }
+            if (share > 1) {
+              float* sums = reinterpret_cast<float*>(smem + warp * kPagedRing + spare * kPagedStageBytes);
+              reinterpret_cast<float4*>(sums)[lane] = acc;
+              if (lane == 0) {
+                piece_ml[warp][0][0] = top;
+                piece_ml[warp][0][1] = sum;
+              }
+              named_sync(1 + r, share * 32);
+              if (turn > 0) continue;
+              for (int x = 1; x < share; ++x) top = fmaxf(top, piece_ml[warp + x][0][0]);
+              acc = make_float4(0.f, 0.f, 0.f, 0.f);
+              sum = 0.f;
+              const float zero = top == -INFINITY ? 0.f : top;
+              for (int x = 0; x < share; ++x) {
+                const float c = exp2f(piece_ml[warp + x][0][0] - zero);
+                const float4 v = *reinterpret_cast<const float4*>(smem + (warp + x) * kPagedRing +
+                                                                  free_slot[warp + x] * kPagedStageBytes + lane * 16);
+                acc = make_float4(acc.x + c * v.x, acc.y + c * v.y, acc.z + c * v.z, acc.w + c * v.w);
+                sum += c * piece_ml[warp + x][0][1];
+              }
+            }
+            RowPlace at;
+            row_place(p, s, w.h, r0 + r, &at);
+            finish_row(p, at, acc, top, sum, lane);
+          }
+        }
+      }
+      __syncthreads();  // the slots that hold the O tiles are the next to be copied to
     }
-    pos += cnt;
-    __syncthreads();  // the joining buffer is the ring of the next piece
+    cp_async_wait<0>();
+    if (pieces - round * kPagedList <= kPagedList) return;
+    __syncthreads();  // the list is written anew
   }
 }
 

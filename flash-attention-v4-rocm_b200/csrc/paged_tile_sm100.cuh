@@ -53,17 +53,18 @@ struct Piece {
 };
 static_assert(sizeof(Piece) == 64, "four 16-byte words");
 
-// sum over j < n of floor((a j + c) / 128), for a, c >= 0
+// sum over j < n of floor((a j + c) / 128), for a, c >= 0, by the steps of Euclid's algorithm
 __host__ __device__ __forceinline__ int64_t floor_sum128(int64_t n, int64_t a, int64_t c) {
-  int64_t m = 128, s = 0;
+  int64_t s = 0, m = 128;
   while (n > 0) {
-    s += n * (n - 1) / 2 * (a / m) + n * (c / m);
-    a %= m;
-    c %= m;
+    const int64_t qa = quotient(a, m), qc = quotient(c, m);
+    s += n * (n - 1) / 2 * qa + n * qc;
+    a -= qa * m;
+    c -= qc * m;
     const int64_t y = a * n + c;
     if (y < m) break;
-    n = y / m;
-    c = y % m;
+    n = quotient(y, m);
+    c = y - n * m;
     const int64_t t = m;
     m = a;
     a = t;
@@ -83,20 +84,20 @@ __host__ __device__ __forceinline__ int unit_steps(const SeqView& s, int causal,
 __host__ __device__ __forceinline__ int64_t units_steps(const SeqView& s, int causal, int bt, int64_t r) {
   if (r <= 0) return 0;
   if (!causal) return r * steps_up_to(s.len);
-  const int64_t units = (static_cast<int64_t>(s.sq) + bt - 1) / bt;
+  const int64_t units = quotient(static_cast<int64_t>(s.sq) + bt - 1, bt);
   int64_t sum = 0;
   if (r == units) {  // the last one ends with the sequence, the others after a whole number of bt tokens
     sum = steps_up_to(s.len);
     --r;
   }
   const int64_t past = static_cast<int64_t>(s.len) - s.sq;
-  int64_t ones = past <= kTileKeys ? (kTileKeys - past) / bt : 0;  // units that end within the first tile
+  int64_t ones = past <= kTileKeys ? quotient(kTileKeys - past, bt) : 0;  // units that end within the first tile
   if (ones > r) ones = r;
   // units ones .. r - 1: ceil((past + (j + 1) bt) / 128)
   return sum + ones + floor_sum128(r - ones, bt, past + (ones + 1) * bt + kTileKeys - 1);
 }
 __host__ __device__ __forceinline__ int64_t tile_seq_work(const SeqView& s, int causal, int bt) {
-  return s.sq == 0 ? 0 : units_steps(s, causal, bt, (static_cast<int64_t>(s.sq) + bt - 1) / bt);
+  return s.sq == 0 ? 0 : units_steps(s, causal, bt, quotient(static_cast<int64_t>(s.sq) + bt - 1, bt));
 }
 
 template <int QTiles>
@@ -202,7 +203,7 @@ __global__ void __launch_bounds__(384, 1)
       }
       if (p.c.batch <= 384) {  // one step sees the whole batch
         total = sum;
-        per = max((total + gridDim.x - 1) / gridDim.x, int64_t(1));
+        per = max(quotient(total + gridDim.x - 1, gridDim.x), int64_t(1));
         begin = blockIdx.x * per;
         pass = 1;
       }
@@ -215,7 +216,7 @@ __global__ void __launch_bounds__(384, 1)
     }
     if (pass == 0) {
       total = base;
-      per = max((total + gridDim.x - 1) / gridDim.x, int64_t(1));
+      per = max(quotient(total + gridDim.x - 1, gridDim.x), int64_t(1));
       begin = blockIdx.x * per;
     }
   }
@@ -489,16 +490,17 @@ __global__ void __launch_bounds__(384, 1)
           ring.advance<Slots>();
         }
       }
-    } else if (lane == 0) {
+    } else {
       // ============================== schedule ==============================
       int4 cut = make_int4(0, 0, 0, -1);
       int out = 0;
-      auto slot_free = [&]() -> bool {
+      bool ok = true;
+      auto put = [&](const Piece& w) {  // lane 0
         const int s = out % kPieceSlots;
-        return mbar_wait(bar(L::kPieceEmpty + s), ((out / kPieceSlots) & 1u) ^ 1u, ctl, kStatusTimeoutLoad);
-      };
-      auto put = [&](const Piece& w) {
-        const int s = out % kPieceSlots;
+        if (!mbar_wait(bar(L::kPieceEmpty + s), ((out / kPieceSlots) & 1u) ^ 1u, ctl, kStatusTimeoutLoad)) {
+          ok = false;
+          return;
+        }
         int4* dst = reinterpret_cast<int4*>(pieces + s);
         dst[0] = make_int4(w.token0, w.tokens, w.past, w.len);
         dst[1] = make_int4(w.h, w.b, w.tile0, w.cnt);
@@ -506,59 +508,65 @@ __global__ void __launch_bounds__(384, 1)
         mbar_arrive(bar(L::kPieceFull + s));  // releases the writes above
         ++out;
       };
-      bool ok = true;
       if (begin < end) {
-        int64_t base = scan[12];
+        int64_t base = scan[12], pos = begin;
         int b = static_cast<int>(scan[13]);
-        int64_t pos = begin;
-        while (pos < end && ok) {
+        while (pos < end) {
           const SeqView s = seq_view(p.c, p.cu, p.total_q, p.max_sq, b);
           const int64_t head_work = tile_seq_work(s, p.causal, bt);
-          const int units = (s.sq + bt - 1) / bt;
           const int64_t stop = min(end, base + head_work * p.c.kv_heads);
           if (pos < stop) {
-            int h = static_cast<int>((pos - base) / head_work);
-            // the unit that holds `pos`: the last r whose earlier units end at or before it
+            const int units = (s.sq + bt - 1) / bt;
+            int h = static_cast<int>(quotient(pos - base, head_work));
+            // the unit that holds `pos`: the last r whose earlier units end at or before it, 32 probes a round
             const int64_t x = pos - base - h * head_work;
-            int lo = 0, hi = units - 1;
-            while (lo < hi) {
-              const int mid = (lo + hi + 1) / 2;
-              if (units_steps(s, p.causal, bt, mid) <= x) lo = mid;
-              else hi = mid - 1;
+            int r = 0, hi = units;  // r fits, hi does not
+            while (hi - r > 1) {
+              const int step = (hi - r + 31) / 32;
+              const int64_t probe = r + static_cast<int64_t>(lane) * step;
+              const bool fits = probe < hi && units_steps(s, p.causal, bt, probe) <= x;
+              const int n = __popc(__ballot_sync(0xffffffffu, fits));  // lane 0 always fits
+              r += (n - 1) * step;
+              hi = min(hi, r + step);
             }
-            int r = lo;
-            int64_t first = base + h * head_work + units_steps(s, p.causal, bt, r);  // the unit's place on the line
-            while (pos < stop) {
-              Piece w;
-              w.n = unit_steps(s, p.causal, bt, r);
-              w.token0 = s.q0 + r * bt;
-              w.tokens = min(bt, s.sq - r * bt);
-              w.past = s.len - s.sq + r * bt;
-              w.len = s.len;
-              w.h = h;
-              w.b = b;
-              w.tile0 = static_cast<int>(pos - first);
-              w.cnt = static_cast<int>(min(static_cast<int64_t>(w.n - w.tile0), end - pos));
-              if (!slot_free()) { ok = false; break; }
-              put(w);
-              if (w.tile0 == 0 && w.cnt < w.n)
-                cut = make_int4(w.token0, w.tokens, h, static_cast<int>((first + w.n - 1) / per));
-              pos += w.cnt;
-              first += w.n;
-              if (++r == units) {
-                r = 0;
-                ++h;
+            if (lane == 0) {
+              int64_t first = base + h * head_work + units_steps(s, p.causal, bt, r);  // the unit's place on the line
+              for (int64_t at = pos; at < stop && ok;) {
+                Piece w;
+                w.n = unit_steps(s, p.causal, bt, r);
+                w.token0 = s.q0 + r * bt;
+                w.tokens = min(bt, s.sq - r * bt);
+                w.past = s.len - s.sq + r * bt;
+                w.len = s.len;
+                w.h = h;
+                w.b = b;
+                w.tile0 = static_cast<int>(at - first);
+                w.cnt = static_cast<int>(min(static_cast<int64_t>(w.n - w.tile0), end - at));
+                put(w);
+                if (w.tile0 == 0 && w.cnt < w.n)
+                  cut = make_int4(w.token0, w.tokens, h, static_cast<int>(quotient(first + w.n - 1, per)));
+                at += w.cnt;
+                first += w.n;
+                if (++r == units) {
+                  r = 0;
+                  ++h;
+                }
               }
             }
+            ok = __all_sync(0xffffffffu, ok);
+            if (!ok) break;
+            pos = stop;
           }
           base += head_work * p.c.kv_heads;
           ++b;
         }
       }
-      tp.cut[blockIdx.x] = cut;
-      if (ok && slot_free()) {
-        Piece w = {};
-        put(w);  // cnt = 0: no more
+      if (lane == 0) {
+        tp.cut[blockIdx.x] = cut;
+        if (ok) {
+          Piece w = {};
+          put(w);  // cnt = 0: no more
+        }
       }
     }
   } else if (warp < 4 * QTiles) {
@@ -623,8 +631,7 @@ __global__ void __launch_bounds__(384, 1)
         const float alpha = rescale ? ((m_new == -INFINITY) ? 1.f : ex2_mufu(m - m_new)) : 1.f;
         m = m_new;
         const float mb = (m == -INFINITY) ? 0.f : m;
-        const float rowsum = masked ? exp_pack_store<0, true>(s, scale_log2, mb, t_s)
-                                    : exp_pack_store<0, false>(s, scale_log2, mb, t_s);
+        const float rowsum = exp_pack_store<0, true>(s, scale_log2, mb, t_s);
         l = l * alpha + rowsum;
         if (rescale) {
           if (QTiles == 1) {  // S runs two steps ahead: P V of the step before may still be at work on O
@@ -673,9 +680,11 @@ __global__ void __launch_bounds__(384, 1)
       if (w.cnt < w.n) {  // a piece: (m, l, O) to the workspace
         const int64_t tile = part_tile(2 * blockIdx.x + (w.tile0 == 0 ? 1 : 0), QTiles, i);
         float4* dst = reinterpret_cast<float4*>(p.part_o) + tile * 4096 + row;
+        if (live) {
 #pragma unroll
-        for (int c = 0; c < 32; ++c) dst[c * 128] = make_float4(ov(4 * c), ov(4 * c + 1), ov(4 * c + 2), ov(4 * c + 3));
-        reinterpret_cast<float2*>(p.part_ml)[tile * 128 + row] = make_float2(m, l);
+          for (int c = 0; c < 32; ++c) dst[c * 128] = make_float4(ov(4 * c), ov(4 * c + 1), ov(4 * c + 2), ov(4 * c + 3));
+          reinterpret_cast<float2*>(p.part_ml)[tile * 128 + row] = make_float2(m, l);
+        }
       } else if (live) {
         const int64_t token = w.token0 + t0 + row_token;
         const int head = w.h * p.group + row_head;
@@ -729,28 +738,130 @@ __global__ void __launch_bounds__(384, 1)
 }
 
 // Adds up the pieces of the units that paged_tile_kernel cut, in key order: O = sum 2^(m_c - M) O_c / L,
-// M = max m_c, L = sum 2^(m_c - M) l_c. Reads each piece once and writes each row once, so L2 bandwidth
-// bounds it; the work items are (unit, Q tile, 4 columns), 128 rows wide, the pieces of each in two
-// halves, so that two units cut into 64 pieces still occupy every SM.
+// M = max m_c, L = sum 2^(m_c - M) l_c. Reads each piece once and writes each row once: L2 traffic, and at
+// small sizes its latency. A work item is a unit's Q tile and C of its 32 column pieces, 128 rows wide, the
+// unit's pieces in two halves; C = 1 gives two units of 64 pieces enough items for every SM, C = 4 keeps
+// more loads in flight where there are many units of few pieces.
+template <int QTiles, int C>
+__device__ __forceinline__ void join_items(const PagedTileParams& tp, const int4* cuts, const int* first_block,
+                                           int count, float4 (*half_o)[128], float2* half_ml) {
+  constexpr int kBatch = 8 / C;  // pieces whose loads are in flight together
+  const PagedParams& p = tp.p;
+  const int row = threadIdx.x % 128, half = threadIdx.x / 128;
+  const int row_token = row / p.group, row_head = row - row_token * p.group;
+  const float4* part_o = reinterpret_cast<const float4*>(p.part_o);
+  const float2* part_ml = reinterpret_cast<const float2*>(p.part_ml);
+  const int items = count * QTiles * (32 / C);
+  for (int item = blockIdx.x; item < items; item += gridDim.x) {
+    const int u = item / (QTiles * (32 / C)), i = item / (32 / C) % QTiles, col = item % (32 / C) * C;
+    const int4 c = cuts[u];
+    const int t0 = i * tp.tile_tokens;
+    if (t0 >= c.y) continue;  // block-uniform
+    const bool live = row_token < tp.tile_tokens && t0 + row_token < c.y;
+    const int c0 = first_block[u], parts = c.w - c0 + 1;
+    const int mid = (parts + 1) / 2, from = half ? mid : 0, to = half ? parts : mid;
+    auto tile = [&](int x) { return part_tile(2 * (c0 + x) + (x == 0 ? 1 : 0), QTiles, i); };
+    float m = -INFINITY, l = 0.f;
+    float4 acc[C];
+#pragma unroll
+    for (int e = 0; e < C; ++e) acc[e] = make_float4(0.f, 0.f, 0.f, 0.f);
+    if (live) {
+      for (int x0 = from; x0 < to; x0 += kBatch) {
+        float2 ml[kBatch];
+        float4 o[kBatch][C];
+#pragma unroll
+        for (int x = 0; x < kBatch; ++x) {
+          if (x0 + x < to) {
+            ml[x] = __ldcg(part_ml + tile(x0 + x) * 128 + row);
+#pragma unroll
+            for (int e = 0; e < C; ++e) o[x][e] = __ldcg(part_o + tile(x0 + x) * 4096 + (col + e) * 128 + row);
+          } else {
+            ml[x] = make_float2(-INFINITY, 0.f);
+#pragma unroll
+            for (int e = 0; e < C; ++e) o[x][e] = make_float4(0.f, 0.f, 0.f, 0.f);
+          }
+        }
+        float top = m;
+#pragma unroll
+        for (int x = 0; x < kBatch; ++x) top = fmaxf(top, ml[x].x);
+        // relative to 0 while no piece has seen a key: NaN sums still go through
+        const float zero = top == -INFINITY ? 0.f : top, a = exp2f(m - zero);
+        l *= a;
+        m = top;
+#pragma unroll
+        for (int e = 0; e < C; ++e) acc[e] = make_float4(acc[e].x * a, acc[e].y * a, acc[e].z * a, acc[e].w * a);
+#pragma unroll
+        for (int x = 0; x < kBatch; ++x) {
+          const float b = exp2f(ml[x].x - zero);
+          l = fmaf(ml[x].y, b, l);
+#pragma unroll
+          for (int e = 0; e < C; ++e)
+            acc[e] = make_float4(fmaf(o[x][e].x, b, acc[e].x), fmaf(o[x][e].y, b, acc[e].y),
+                                 fmaf(o[x][e].z, b, acc[e].z), fmaf(o[x][e].w, b, acc[e].w));
+        }
+      }
+    }
+    if (half) {
+#pragma unroll
+      for (int e = 0; e < C; ++e) half_o[e][row] = acc[e];
+      half_ml[row] = make_float2(m, l);
+    }
+    __syncthreads();
+    if (!half && live) {
+      const int64_t token = c.x + t0 + row_token;
+      const int head = c.z * p.group + row_head;
+      const int64_t orow = token * p.heads + head, lse_at = static_cast<int64_t>(head) * p.total_q + token;
+      const float2 ml = half_ml[row];
+      const float other = p.add_o != nullptr ? __ldcg(p.add_lse + lse_at) * 1.4426950408889634f : -INFINITY;
+      const float top = fmax3(m, ml.x, other);
+      const bool any = top != -INFINITY;
+      float a = any ? exp2f(m - top) : 0.f, b = any ? exp2f(ml.x - top) : 0.f, x = any ? exp2f(other - top) : 0.f;
+      l = l * a + ml.y * b + x;
+      const float inv = l == 0.f ? 0.f : 1.f / l;
+      a *= inv;
+      b *= inv;
+      x *= inv;
+#pragma unroll
+      for (int e = 0; e < C; ++e) {
+        const float4 o = half_o[e][row];
+        float4 v = make_float4(acc[e].x * a + o.x * b, acc[e].y * a + o.y * b, acc[e].z * a + o.z * b, acc[e].w * a + o.w * b);
+        if (p.add_o != nullptr) {
+          const float4 f = __ldcg(reinterpret_cast<const float4*>(p.add_o + orow * 128) + col + e);
+          v = make_float4(fmaf(f.x, x, v.x), fmaf(f.y, x, v.y), fmaf(f.z, x, v.z), fmaf(f.w, x, v.w));
+        }
+        if (p.o != nullptr)
+          *reinterpret_cast<uint2*>(p.o + orow * 128 + (col + e) * 4) =
+              make_uint2(pack_bf16x2(v.x, v.y), pack_bf16x2(v.z, v.w));
+        else
+          reinterpret_cast<float4*>(p.o32 + orow * 128)[col + e] = v;
+      }
+      if (p.lse != nullptr && col == 0) p.lse[lse_at] = l == 0.f ? -INFINITY : top * kLn2 + logf(l);
+    }
+    __syncthreads();
+  }
+}
+
+constexpr int kJoinPerSm = 4;
+
 template <int QTiles>
-__global__ void __launch_bounds__(256) paged_join_kernel(const __grid_constant__ PagedTileParams tp, int blocks) {
+__global__ void __launch_bounds__(256, kJoinPerSm) paged_join_kernel(const __grid_constant__ PagedTileParams tp, int blocks) {
   constexpr int kMaxCuts = 256;
   __shared__ int4 cuts[kMaxCuts];
   __shared__ int first_block[kMaxCuts];
   __shared__ int warp_cuts[kMaxCuts / 32];
-  __shared__ float4 half_o[128];
+  __shared__ float4 half_o[4][128];
   __shared__ float2 half_ml[128];
-  const PagedParams& p = tp.p;
   asm volatile("griddepcontrol.wait;" ::: "memory");
   // the cut units, numbered alike in every block: by the block that opens them (blocks <= kMaxCuts threads)
+  const int warp = threadIdx.x / 32;
   const int4 mine = static_cast<int>(threadIdx.x) < blocks ? __ldcg(tp.cut + threadIdx.x) : make_int4(0, 0, 0, -1);
   const uint32_t opens = __ballot_sync(0xffffffffu, mine.w >= 0);
-  if (threadIdx.x % 32 == 0) warp_cuts[threadIdx.x / 32] = __popc(opens);
+  if (threadIdx.x % 32 == 0) warp_cuts[warp] = __popc(opens);
   __syncthreads();
   int at = __popc(opens & ((1u << (threadIdx.x % 32)) - 1)), count = 0;
 #pragma unroll
   for (int w = 0; w < kMaxCuts / 32; ++w) {
-    if (w < static_cast<int>(threadIdx.x / 32)) at += warp_cuts[w];
+    if (w < warp) at += warp_cuts[w];
     count += warp_cuts[w];
   }
   if (mine.w >= 0) {
@@ -758,85 +869,10 @@ __global__ void __launch_bounds__(256) paged_join_kernel(const __grid_constant__
     first_block[at] = threadIdx.x;
   }
   __syncthreads();
-  const int row = threadIdx.x % 128, half = threadIdx.x / 128;
-  const int row_token = row / p.group, row_head = row - row_token * p.group;
-  const float4* part_o = reinterpret_cast<const float4*>(p.part_o);
-  const float2* part_ml = reinterpret_cast<const float2*>(p.part_ml);
-  const int items = count * QTiles * 32;
-  for (int item = blockIdx.x; item < items; item += gridDim.x) {
-    const int u = item / (QTiles * 32), i = item / 32 % QTiles, col = item % 32;
-    const int4 c = cuts[u];
-    const int t0 = i * tp.tile_tokens;
-    if (t0 >= c.y) continue;  // block-uniform
-    const int c0 = first_block[u], parts = c.w - c0 + 1;
-    const int mid = (parts + 1) / 2, from = half ? mid : 0, to = half ? parts : mid;
-    auto tile = [&](int x) { return part_tile(2 * (c0 + x) + (x == 0 ? 1 : 0), QTiles, i); };
-    float m = -INFINITY, l = 0.f;
-    float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
-    for (int x0 = from; x0 < to; x0 += 8) {
-      float2 ml[8];
-      float4 o[8];
-#pragma unroll
-      for (int x = 0; x < 8; ++x) {
-        if (x0 + x < to) {
-          ml[x] = __ldcg(part_ml + tile(x0 + x) * 128 + row);
-          o[x] = __ldcg(part_o + tile(x0 + x) * 4096 + col * 128 + row);
-        } else {
-          ml[x] = make_float2(-INFINITY, 0.f);
-          o[x] = make_float4(0.f, 0.f, 0.f, 0.f);
-        }
-      }
-      float top = m;
-#pragma unroll
-      for (int x = 0; x < 8; ++x) top = fmaxf(top, ml[x].x);
-      if (top != -INFINITY) {
-        const float a = exp2f(m - top);
-        acc = make_float4(acc.x * a, acc.y * a, acc.z * a, acc.w * a);
-        l *= a;
-        m = top;
-#pragma unroll
-        for (int x = 0; x < 8; ++x) {
-          const float b = exp2f(ml[x].x - top);
-          acc = make_float4(fmaf(o[x].x, b, acc.x), fmaf(o[x].y, b, acc.y), fmaf(o[x].z, b, acc.z), fmaf(o[x].w, b, acc.w));
-          l = fmaf(ml[x].y, b, l);
-        }
-      }
-    }
-    if (half) {
-      half_o[row] = acc;
-      half_ml[row] = make_float2(m, l);
-    }
-    __syncthreads();
-    if (!half && row_token < tp.tile_tokens && t0 + row_token < c.y) {
-      const int64_t token = c.x + t0 + row_token;
-      const int head = c.z * p.group + row_head;
-      const int64_t orow = token * p.heads + head, lse_at = static_cast<int64_t>(head) * p.total_q + token;
-      const float2 ml = half_ml[row];
-      const float4 o = half_o[row];
-      float other = -INFINITY;
-      float4 e = make_float4(0.f, 0.f, 0.f, 0.f);
-      if (p.add_o != nullptr) {
-        other = __ldcg(p.add_lse + lse_at) * 1.4426950408889634f;
-        e = __ldcg(reinterpret_cast<const float4*>(p.add_o + orow * 128) + col);
-      }
-      const float top = fmax3(m, ml.x, other);
-      if (top != -INFINITY) {
-        const float a = exp2f(m - top), b = exp2f(ml.x - top), x = exp2f(other - top);
-        l = l * a + ml.y * b + x;
-        acc = make_float4(acc.x * a + o.x * b + e.x * x, acc.y * a + o.y * b + e.y * x, acc.z * a + o.z * b + e.z * x,
-                          acc.w * a + o.w * b + e.w * x);
-        m = top;
-      }
-      const float inv = l == 0.f ? 0.f : 1.f / l;
-      acc = make_float4(acc.x * inv, acc.y * inv, acc.z * inv, acc.w * inv);
-      if (p.o != nullptr)
-        *reinterpret_cast<uint2*>(p.o + orow * 128 + col * 4) = make_uint2(pack_bf16x2(acc.x, acc.y), pack_bf16x2(acc.z, acc.w));
-      else
-        reinterpret_cast<float4*>(p.o32 + orow * 128)[col] = acc;
-      if (p.lse != nullptr && col == 0) p.lse[lse_at] = l == 0.f ? -INFINITY : m * kLn2 + logf(l);
-    }
-    __syncthreads();
-  }
+  if (count * QTiles * 32 > 2 * static_cast<int>(gridDim.x))
+    join_items<QTiles, 4>(tp, cuts, first_block, count, half_o, half_ml);
+  else
+    join_items<QTiles, 1>(tp, cuts, first_block, count, half_o, half_ml);
 }
 
 }  // namespace fav4

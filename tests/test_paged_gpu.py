@@ -426,3 +426,23 @@ def test_two_graphs_and_eager_calls_do_not_share_a_workspace(cuda):
     torch.cuda.synchronize()
     for got, ref in (*zip(outs, want), (eager, want[0])):
         assert torch.equal(got[0], ref[0]) and torch.equal(got[1], ref[1])
+
+
+@pytest.mark.parametrize("sq,keys", [([1, 1], [5000, 5000]), ([40, 40], [5000, 5000])])
+def test_nan_query_shows_in_its_rows_only(cuda, sq, keys):
+    # also where a row's keys are split over many blocks
+    x = Batch(sq, keys, 4, 2, 16, seed=53)
+    x.q[0, 1] = float("nan")
+    o, lse = attend(x)
+    assert torch.isnan(o[0, 1]).all() and torch.isnan(lse[1, 0])
+    o[0, 1], lse[1, 0] = 0, 0
+    assert torch.isfinite(o).all() and torch.isfinite(lse).all()
+
+
+def test_many_short_sequences(cuda):
+    # more sequences than one scan step, and blocks whose stretch has more pieces than are listed at a time
+    b = 4500
+    keys = [1 + i % 3 for i in range(b)]
+    x = Batch([1] * b, keys, 8, 8, 16, seed=54)
+    o, lse = attend(x)
+    check_attention(o, lse, x.reference())
