@@ -21,6 +21,22 @@ constexpr int kMaxSms = 160;         // bound on the SMs that the workspace is l
 constexpr int kPagedPerSm = 2;       // blocks of paged_attn_kernel per SM
 constexpr int kMaxGrid = kMaxSms * kPagedPerSm;
 
+// Launch as a programmatic dependent (see wait_for_predecessor).
+template <typename... Params, typename... Args>
+int launch(void (*kernel)(Params...), unsigned grid, unsigned block, size_t smem, cudaStream_t stream, Args&&... args) {
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3(grid);
+  cfg.blockDim = dim3(block);
+  cfg.dynamicSmemBytes = smem;
+  cfg.stream = stream;
+  cudaLaunchAttribute attr[1];
+  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[0].val.programmaticStreamSerializationAllowed = 1;
+  cfg.attrs = attr;
+  cfg.numAttrs = 1;
+  return cudaLaunchKernelEx(&cfg, kernel, args...);
+}
+
 bool aligned16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15) == 0; }
 bool aligned4(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 3) == 0; }
 bool stride_ok(long long s) { return s >= 0 && s % 8 == 0; }
@@ -170,19 +186,9 @@ int launch_tiles(const PagedParams& p, const PagedSpace& sp, uint8_t* ws, int sm
   if (!encode_rows(&tq, p.q, 3, dims, strides, box) || !encode_cache(&tk, p.c.k, p.c, t.box_rows) ||
       !encode_cache(&tv, p.c.v, p.c, t.box_rows))
     return cudaErrorInvalidValue;
-  paged_tile_kernel<QTiles><<<sms, 384, PagedTileLayout<QTiles>::kAlloc, stream>>>(tq, tk, tv, t);
-  if (cudaError_t e = cudaGetLastError(); e != cudaSuccess) return e;
-  // the join goes out as a programmatic dependent launch: it waits for the pieces itself
-  cudaLaunchConfig_t cfg = {};
-  cfg.gridDim = dim3(kJoinPerSm * sms);
-  cfg.blockDim = dim3(256);
-  cfg.stream = stream;
-  cudaLaunchAttribute attr[1];
-  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
-  attr[0].val.programmaticStreamSerializationAllowed = 1;
-  cfg.attrs = attr;
-  cfg.numAttrs = 1;
-  return cudaLaunchKernelEx(&cfg, paged_join_kernel<QTiles>, t, sms);
+  const int rc = launch(paged_tile_kernel<QTiles>, sms, 384, PagedTileLayout<QTiles>::kAlloc, stream, tq, tk, tv, t);
+  if (rc) return rc;
+  return launch(paged_join_kernel<QTiles>, kJoinPerSm * sms, 256, 0, stream, t, sms);
 }
 
 // One attention of all rows over one set of page tables.
@@ -193,8 +199,7 @@ int launch_rows(const PagedParams& p, const PagedSpace& sp, uint8_t* ws, int sms
   const int tiles = mapped ? q_tiles(p.max_sq, p.group) : 0;
   if (tiles == 1) return launch_tiles<1>(p, sp, ws, sms, stream);
   if (tiles == 2) return launch_tiles<2>(p, sp, ws, sms, stream);
-  paged_attn_kernel<<<sms * kPagedPerSm, kPagedWarps * 32, kPagedSmem, stream>>>(p);
-  return cudaGetLastError();
+  return launch(paged_attn_kernel, sms * kPagedPerSm, kPagedWarps * 32, kPagedSmem, stream, p);
 }
 
 int launch_paged(const Fav4PagedArgs& a, int causal, uint8_t* ws, cudaStream_t stream) {
@@ -280,9 +285,8 @@ extern "C" int fav4_bshd_paged_append(const Fav4PagedAppendArgs* a, cudaStream_t
   const long long per_token = (a->heads + 2ll * a->cache.kv_heads + fav4::kAppendRows - 1) / fav4::kAppendRows;
   const long long blocks = (a->total_q * per_token + 7) / 8;
   if (blocks > INT_MAX) return cudaErrorInvalidValue;
-  auto kernel = a->interleaved ? fav4::paged_append_kernel<true> : fav4::paged_append_kernel<false>;
-  kernel<<<static_cast<unsigned>(blocks), 256, 0, stream>>>(p);
-  return cudaGetLastError();
+  return fav4::launch(a->interleaved ? fav4::paged_append_kernel<true> : fav4::paged_append_kernel<false>,
+                      static_cast<unsigned>(blocks), 256, 0, stream, p);
 }
 
 extern "C" size_t fav4_bshd_paged_workspace_bytes(const Fav4PagedArgs* a) {

@@ -12,6 +12,14 @@
 
 namespace fav4 {
 
+// Every kernel here is launched as a programmatic dependent of whatever precedes it on its stream: it may be
+// scheduled while that still runs, waits here before it reads or writes any memory that others use, and
+// lets its own successor be scheduled at once.
+__device__ __forceinline__ void wait_for_predecessor() {
+  asm volatile("griddepcontrol.wait;" ::: "memory");
+  asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
+}
+
 struct PagedCacheView {
   __nv_bfloat16 *k, *v;
   int64_t page_stride, token_stride, head_stride;  // elements
@@ -100,6 +108,7 @@ __global__ void __launch_bounds__(256) paged_append_kernel(const __grid_constant
   const int hk = p.c.kv_heads, rows = p.heads + 2 * hk;
   const int per_token = (rows + kAppendRows - 1) / kAppendRows;
   const int64_t item = (static_cast<int64_t>(blockIdx.x) * blockDim.x + threadIdx.x) / 32;
+  wait_for_predecessor();
   if (item >= static_cast<int64_t>(p.total_q) * per_token) return;
   const int t = static_cast<int>(item / per_token);
   const int r0 = static_cast<int>(item - static_cast<int64_t>(t) * per_token) * kAppendRows;
@@ -362,6 +371,7 @@ __global__ void __launch_bounds__(kPagedWarps * 32, 2) paged_attn_kernel(const _
   const int mi = lane / 8, mr = lane % 8;    // ldmatrix: matrix and row that this lane addresses
   const int cl = lane % 16, rl = lane / 16;  // copies: 16-byte piece cl of rows rl + 2 j
   const uint32_t ring = smem_addr(smem) + warp * kPagedRing;
+  wait_for_predecessor();
 
   int64_t total = 0, per = 0, begin = 0, end = 0;
   for (int round = 0;; ++round) {
@@ -532,17 +542,19 @@ __global__ void __launch_bounds__(kPagedWarps * 32, 2) paged_attn_kernel(const _
       for (int st_i = 0; st_i < steps; ++st_i, key += kPagedWarps * 16) {
         cp_async_wait<kPagedStages - 2>();
         __syncwarp();  // this group has arrived, and every lane is done with the one before
-        issue();
         const uint32_t st = ring + slot * kPagedStageBytes;
         slot = slot == kPagedStages - 1 ? 0 : slot + 1;
-        float sc[2][4] = {};
+        float sc[2][4] = {}, sc_odd[2][4] = {};  // two chains each: a chain of eight products would show
 #pragma unroll
         for (int k = 0; k < 8; ++k) {
           uint32_t kb[4];
           ldsm4(st + ((mi / 2) * 8 + mr) * 256 + (((2 * k + (mi & 1)) ^ mr) * 16), kb);
-          mma16816(sc[0], qf[k], kb[0], kb[1]);
-          mma16816(sc[1], qf[k], kb[2], kb[3]);
+          mma16816(k & 1 ? sc_odd[0] : sc[0], qf[k], kb[0], kb[1]);
+          mma16816(k & 1 ? sc_odd[1] : sc[1], qf[k], kb[2], kb[3]);
         }
+        issue();  // behind the products
+#pragma unroll
+        for (int e = 0; e < 8; ++e) sc[e / 4][e % 4] += sc_odd[e / 4][e % 4];
         if (key + 15 > lim_min) {
 #pragma unroll
           for (int e = 0; e < 8; ++e) {

@@ -177,7 +177,7 @@ __global__ void __launch_bounds__(384, 1)
     tmem_alloc(smem_addr(tmem_holder), 512);
     tmem_relinquish();
   }
-  asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
+  wait_for_predecessor();
 
   // ---- this block's stretch of the line of steps, and the sequence that it begins in ----
   const int bt = tp.tile_tokens * QTiles;
@@ -691,7 +691,6 @@ __global__ void __launch_bounds__(384, 1)
         const int64_t orow = token * p.heads + head, lse_at = static_cast<int64_t>(head) * p.total_q + token;
         float a = 1.f, x = 0.f;
         if (p.add_o != nullptr) {  // the other result of this row, joined in
-          asm volatile("griddepcontrol.wait;" ::: "memory");
           const float other = __ldcg(p.add_lse + lse_at) * 1.4426950408889634f;
           const float top = fmaxf(m, other);
           if (top != -INFINITY) {
@@ -851,7 +850,7 @@ __global__ void __launch_bounds__(256, kJoinPerSm) paged_join_kernel(const __gri
   __shared__ int warp_cuts[kMaxCuts / 32];
   __shared__ float4 half_o[4][128];
   __shared__ float2 half_ml[128];
-  asm volatile("griddepcontrol.wait;" ::: "memory");
+  wait_for_predecessor();
   // the cut units, numbered alike in every block: by the block that opens them (blocks <= kMaxCuts threads)
   const int warp = threadIdx.x / 32;
   const int4 mine = static_cast<int>(threadIdx.x) < blocks ? __ldcg(tp.cut + threadIdx.x) : make_int4(0, 0, 0, -1);
