@@ -9,7 +9,8 @@
 // A block is the warp-specialised pipeline of the contiguous kernel (attn_fwd_sm100.cuh; the TMEM
 // layout, the order of the MMAs, the softmax and its lazy rescaling are described there):
 //
-//   warps 0-3 / 4-7  softmax, correction and epilogue of Q tile 0 / 1, one row per thread
+//   warps 0-3 / 4-7  softmax, correction and epilogue, one row per thread: of Q tile 0 / 1, or of the even /
+//                    odd steps of the only Q tile
 //   warp 8           TMA: Q tiles, then the K/V ring; the lanes hold the page numbers of a tile's groups of
 //                    box_rows keys (a power of two that divides the page size) and each issues its own boxes
 //   warp 9           one thread issues every tcgen05.mma
@@ -53,21 +54,25 @@ struct Piece {
 };
 static_assert(sizeof(Piece) == 64, "four 16-byte words");
 
-// sum over j < n of floor((a j + c) / 128), for a, c >= 0, by the steps of Euclid's algorithm
+// sum over j < n of floor((a j + c) / 128), for a, c >= 0, by the steps of Euclid's algorithm. Blocks wait
+// for it, so the first step (by 128) has no division and the others one each: their c and a are below 128.
 __host__ __device__ __forceinline__ int64_t floor_sum128(int64_t n, int64_t a, int64_t c) {
-  int64_t s = 0, m = 128;
-  while (n > 0) {
-    const int64_t qa = quotient(a, m), qc = quotient(c, m);
-    s += n * (n - 1) / 2 * qa + n * qc;
-    a -= qa * m;
-    c -= qc * m;
-    const int64_t y = a * n + c;
+  if (n <= 0) return 0;
+  int64_t s = n * (n - 1) / 2 * (a >> 7) + n * (c >> 7);
+  int m = 128, r = static_cast<int>(a & 127), d = static_cast<int>(c & 127);
+  while (true) {
+    const int64_t y = r * n + d;
     if (y < m) break;
-    n = quotient(y, m);
-    c = y - n * m;
-    const int64_t t = m;
-    m = a;
-    a = t;
+    const int64_t k = m == 128 ? y >> 7 : quotient(y, m);
+    d = static_cast<int>(y - k * m);
+    n = k;
+    const int q = static_cast<int>(static_cast<unsigned>(m) / static_cast<unsigned>(r));  // r > 0: y >= m > d
+    const int e = static_cast<int>(static_cast<unsigned>(d) / static_cast<unsigned>(r));
+    s += n * (n - 1) / 2 * q + n * e;
+    const int t = m - q * r;
+    d -= e * r;
+    m = r;
+    r = t;
   }
   return s;
 }
@@ -115,8 +120,9 @@ struct PagedTileLayout {
   static constexpr int kPieces = (kBar + kNumBars * 8 + 15) & ~15;
   static constexpr int kMisc = kPieces + kPieceSlots * 64;  // TMEM base, abort flag, schedule scan
   static constexpr int kScan = (kMisc + 8 + 15) & ~15;      // 12 warps' sums, then base, sequence
-  static constexpr int kBytes = kScan + 16 * 8;
-  static constexpr int kAlloc = kBytes + 1024;
+  static constexpr int kMl = kScan + 20 * 8;  // one Q tile: (m, l) of the two key streams
+  static constexpr int kBytes = kMl + (QTiles == 1 ? 2 * 128 * 8 : 0);
+  static constexpr int kAlloc = kBytes;  // the kernel checks that its base is 1 KiB aligned
   static_assert(kAlloc <= 227 * 1024, "shared memory budget");
 };
 
@@ -132,9 +138,12 @@ __global__ void __launch_bounds__(384, 1)
   constexpr int Slots = L::kSlots;
   constexpr int KA = QTiles == 1 ? 2 : 1;  // S runs this many steps ahead of P V
   const PagedParams& p = tp.p;
-  extern __shared__ uint8_t smem_raw[];
-  uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
+  extern __shared__ __align__(1024) uint8_t smem[];
   const uint32_t sbase = smem_addr(smem);
+  if (sbase & 1023) {  // the swizzled tiles need it; there is no room to round up
+    if (threadIdx.x == 0) atomicOr(tp.status, kStatusSmemAlign);
+    return;
+  }
   const uint32_t bar0 = sbase + L::kBar;
   auto bar = [&](int slot) -> uint32_t { return bar0 + 8u * slot; };
   uint32_t* tmem_holder = reinterpret_cast<uint32_t*>(smem + L::kMisc);
@@ -159,11 +168,11 @@ __global__ void __launch_bounds__(384, 1)
       mbar_init(bar(L::kSFull + i), 1);
       mbar_init(bar(L::kPFull + i), 4);
       mbar_init(bar(L::kOFull + i), 1);
-      mbar_init(bar(L::kOEmpty + i), 4);
+      mbar_init(bar(L::kOEmpty + i), QTiles == 1 ? 8 : 4);  // the warps that read O_i
     }
     for (int s = 0; s < kPieceSlots; ++s) {
       mbar_init(bar(L::kPieceFull + s), 1);
-      mbar_init(bar(L::kPieceEmpty + s), 3 + 4 * QTiles);  // load, MMA and V warps, softmax warps
+      mbar_init(bar(L::kPieceEmpty + s), 3 + 8);  // load, MMA and V warps, softmax warps
     }
     mbar_init(bar(L::kTeardown), 1);
     fence_mbar_init();
@@ -186,9 +195,10 @@ __global__ void __launch_bounds__(384, 1)
     int64_t base = 0;
     for (int b0 = 0; b0 < p.c.batch; b0 += 384) {
       const int b = b0 + threadIdx.x;
-      int64_t v = 0;
-      if (b < p.c.batch) v = tile_seq_work(seq_view(p.c, p.cu, p.total_q, p.max_sq, b), p.causal, bt) * p.c.kv_heads;
-      const int64_t mine = v;
+      SeqView view = {0, 0, 0};
+      if (b < p.c.batch) view = seq_view(p.c, p.cu, p.total_q, p.max_sq, b);
+      const int64_t head_work = tile_seq_work(view, p.causal, bt), mine = head_work * p.c.kv_heads;
+      int64_t v = mine;
 #pragma unroll
       for (int o = 1; o < 32; o *= 2) {
         const int64_t up = __shfl_up_sync(0xffffffffu, v, o);
@@ -210,6 +220,10 @@ __global__ void __launch_bounds__(384, 1)
       if (pass == 1 && base + v - mine <= begin && begin < base + v) {
         scan[12] = base + v - mine;
         scan[13] = b;
+        scan[14] = head_work;
+        scan[15] = view.q0;
+        scan[16] = view.sq;
+        scan[17] = view.len;
       }
       base += sum;
       __syncthreads();
@@ -254,10 +268,9 @@ __global__ void __launch_bounds__(384, 1)
   };
 
   static_assert(128 * (2 * kTileSoftmaxRegs + kTileOtherRegs) <= 384 * kLaunchRegs, "register split exceeds the launch");
-  static_assert(128 * (kSoftmaxRegs1 + kOtherRegs + kOtherRegs1) <= 384 * kLaunchRegs, "register split exceeds the launch");
 
   if (warp >= 8) {
-    regs_release<(QTiles == 1 ? kOtherRegs1 : kTileOtherRegs)>();
+    regs_release<kTileOtherRegs>();
     if (warp == 8) {
       // ============================ TMA producer ============================
       const uint64_t pol_kv = policy_evict_last();
@@ -344,7 +357,7 @@ __global__ void __launch_bounds__(384, 1)
       const uint64_t dv = make_sdesc_sw128(sbase, kBoxBytes, 1024);
       const uint32_t k_lo = static_cast<uint32_t>(dk), k_hi = static_cast<uint32_t>(dk >> 32);
       const uint32_t v_lo = static_cast<uint32_t>(dv), v_hi = static_cast<uint32_t>(dv >> 32);
-      // S = Q_i K^T into TMEM columns 128 s; O_i += P V, P at columns 128 s
+      // S = Q_i K^T into TMEM columns 128 s; O_o += P V, P at columns 128 s
       auto issue_s = [&](int i, int s, int slot) {
         const uint32_t qa = k_lo + ((L::kQ + i * kTileBytes) >> 4);
         const uint32_t ka = k_lo + ((L::kKV + slot * L::kSlotBytes + kTileBytes) >> 4);
@@ -356,9 +369,9 @@ __global__ void __launch_bounds__(384, 1)
         }
         tc_commit(bar(L::kSFull + s));
       };
-      auto issue_pv = [&](int i, int s, int slot, bool acc) {
+      auto issue_pv = [&](int o, int s, int slot, bool acc) {
         const uint32_t va = v_lo + ((L::kKV + slot * L::kSlotBytes) >> 4);
-        const uint32_t d = tmem + 256 + i * 128, pa = tmem + s * 128;
+        const uint32_t d = tmem + 256 + o * 128, pa = tmem + s * 128;
         umma_ts_w(d, pa, va, v_hi, idesc_pv, acc ? 1u : 0u);
 #pragma unroll
         for (int k = 1; k < kTileKeys / 16; ++k) umma_ts_w(d, pa + k * 8, va + ((k * 2048) >> 4), v_hi, idesc_pv, 1u);
@@ -379,7 +392,7 @@ __global__ void __launch_bounds__(384, 1)
           if (!mbar_wait(bar(L::kQFull), par.q_full(), ctl, kStatusTimeoutMma)) ok = false;
           par.flip_q_full();
           if constexpr (QTiles == 1) {
-            // S buffers j % 2; every P V is committed to pv_done (the o_full barrier of the second tile)
+            // two key streams: step j goes through S buffer j % 2 into O_(j % 2)
             for (int pb = 0; pb < 2 && pb < N && ok; ++pb) {
               if (!mbar_wait(bar(L::kKVFull + ring.stage), ring.phase, ctl, kStatusTimeoutMma)) { ok = false; break; }
               tc_fence_after();
@@ -393,15 +406,14 @@ __global__ void __launch_bounds__(384, 1)
               const int b = j & 1, cur = ring.stage;
               if (!mbar_wait(bar(L::kPFull + b), par.p_full(b), ctl, kStatusTimeoutMma)) { ok = false; break; }
               par.flip_p_full(b);
-              if (j == 0) {
-                if (!mbar_wait(bar(L::kOEmpty), par.o_empty(0), ctl, kStatusTimeoutMma)) { ok = false; break; }
-                par.flip_o_empty(0);
+              if (j < 2) {
+                if (!mbar_wait(bar(L::kOEmpty + b), par.o_empty(b), ctl, kStatusTimeoutMma)) { ok = false; break; }
+                par.flip_o_empty(b);
               }
               if (ragged && j + 1 == N && !wait_fix(cur)) { ok = false; break; }
               tc_fence_after();
-              issue_pv(0, b, cur, j > 0);
-              tc_commit(bar(L::kOFull + 1));
-              if (j + 1 == N) tc_commit(bar(L::kOFull));
+              issue_pv(b, b, cur, j > 1);
+              if (j + 2 >= N) tc_commit(bar(L::kOFull + b));
               if (j + 2 < N) issue_s(0, b, cur);
               tc_commit(bar(L::kKVEmpty + cur));
               if (j + 3 == N) tc_commit(bar(L::kQEmpty));
@@ -511,9 +523,9 @@ __global__ void __launch_bounds__(384, 1)
       if (begin < end) {
         int64_t base = scan[12], pos = begin;
         int b = static_cast<int>(scan[13]);
-        while (pos < end) {
-          const SeqView s = seq_view(p.c, p.cu, p.total_q, p.max_sq, b);
-          const int64_t head_work = tile_seq_work(s, p.causal, bt);
+        SeqView s = {static_cast<int>(scan[15]), static_cast<int>(scan[16]), static_cast<int>(scan[17])};
+        int64_t head_work = scan[14];
+        while (true) {
           const int64_t stop = min(end, base + head_work * p.c.kv_heads);
           if (pos < stop) {
             const int units = (s.sq + bt - 1) / bt;
@@ -521,16 +533,18 @@ __global__ void __launch_bounds__(384, 1)
             // the unit that holds `pos`: the last r whose earlier units end at or before it, 32 probes a round
             const int64_t x = pos - base - h * head_work;
             int r = 0, hi = units;  // r fits, hi does not
+            int64_t before = 0;     // steps of the units before r
             while (hi - r > 1) {
               const int step = (hi - r + 31) / 32;
               const int64_t probe = r + static_cast<int64_t>(lane) * step;
-              const bool fits = probe < hi && units_steps(s, p.causal, bt, probe) <= x;
-              const int n = __popc(__ballot_sync(0xffffffffu, fits));  // lane 0 always fits
+              const int64_t sum = probe < hi ? units_steps(s, p.causal, bt, probe) : 0;
+              const int n = __popc(__ballot_sync(0xffffffffu, probe < hi && sum <= x));  // lane 0 always fits
+              before = __shfl_sync(0xffffffffu, sum, n - 1);
               r += (n - 1) * step;
               hi = min(hi, r + step);
             }
             if (lane == 0) {
-              int64_t first = base + h * head_work + units_steps(s, p.causal, bt, r);  // the unit's place on the line
+              int64_t first = base + h * head_work + before;  // the unit's place on the line
               for (int64_t at = pos; at < stop && ok;) {
                 Piece w;
                 w.n = unit_steps(s, p.causal, bt, r);
@@ -557,8 +571,11 @@ __global__ void __launch_bounds__(384, 1)
             if (!ok) break;
             pos = stop;
           }
+          if (pos >= end) break;
           base += head_work * p.c.kv_heads;
           ++b;
+          s = seq_view(p.c, p.cu, p.total_q, p.max_sq, b);
+          head_work = tile_seq_work(s, p.causal, bt);
         }
       }
       if (lane == 0) {
@@ -569,34 +586,39 @@ __global__ void __launch_bounds__(384, 1)
         }
       }
     }
-  } else if (warp < 4 * QTiles) {
+  } else {
     // ============================== softmax ===============================
-    regs_claim<(QTiles == 1 ? kSoftmaxRegs1 : kTileSoftmaxRegs)>();
+    // Two Q tiles: warpgroup i has tile i. One Q tile: warpgroup i has the tile's steps i, i + 2, ... with an
+    // m, l and O of its own, which both warpgroups join at the end of the piece, 64 columns each.
+    regs_claim<kTileSoftmaxRegs>();
+    constexpr int kStreams = QTiles == 1 ? 2 : 1;
+    constexpr int kCols = 128 / kStreams;  // columns of O that this thread finishes
     const int i = warp / 4;
+    const int tile = QTiles == 1 ? 0 : i;
     const int row = (warp % 4) * 32 + lane;
     const uint32_t lane_off = static_cast<uint32_t>((warp % 4) * 32) << 16;
-    const uint32_t t_s0 = tmem + lane_off + i * 128;
+    const uint32_t t_s = tmem + lane_off + i * 128;
     const uint32_t t_o = tmem + lane_off + 256 + i * 128;
-    uint32_t s_par = 0, o_full_par = 0, pv_seen = 0;
+    const int col0 = QTiles == 1 ? i * kCols : 0;
+    float2* ml_shared = reinterpret_cast<float2*>(smem + L::kMl);  // [stream][row]
+    uint32_t s_par = 0, o_full_par = 0;  // o_full: bit x for O_x
     const float scale_log2 = p.scale_log2;
-    const int row_token = row / p.group;                    // token of this row within the Q tile
+    const int row_token = row / p.group;  // token of this row within the Q tile
     const int row_head = row - row_token * p.group;
     bool ok = true;
     Piece w;
     while (ok && next_piece(&w)) {
-      const int t0 = i * tp.tile_tokens;
+      const int t0 = tile * tp.tile_tokens;
       if (t0 >= w.tokens) continue;  // no rows in this Q tile
-      const int ni = tile_steps(w, i);
+      const int ni = tile_steps(w, tile);
       const bool live = row_token < tp.tile_tokens && t0 + row_token < w.tokens;
-      const int first_lim = p.causal ? w.past + t0 : w.len - 1;                 // last visible key of the tile's first row
-      const int lim_row = p.causal ? w.past + t0 + row_token : w.len - 1;       // and of this one
+      const int first_lim = p.causal ? w.past + t0 : w.len - 1;            // last visible key of the tile's first row
+      const int lim_row = p.causal ? w.past + t0 + row_token : w.len - 1;  // and of this one
+      const int j0 = QTiles == 1 ? i : 0;
       float m = -INFINITY, l = 0.f;
-      for (int j = 0; j < ni; ++j) {
-        const int sb = QTiles == 1 ? (j & 1) : i;
-        const uint32_t t_s = t_s0 + (QTiles == 1 ? sb * 128 : 0);
-        const uint32_t s_bit = QTiles == 1 ? 1u << sb : 1u;
-        if (!warp_wait(bar(L::kSFull + sb), (s_par & s_bit) ? 1u : 0u, ctl, kStatusTimeoutSoftmax)) { ok = false; break; }
-        s_par ^= s_bit;
+      for (int j = j0; j < ni; j += kStreams) {
+        if (!warp_wait(bar(L::kSFull + i), s_par, ctl, kStatusTimeoutSoftmax)) { ok = false; break; }
+        s_par ^= 1u;
         tc_fence_after();
         uint32_t sr[4][32];
 #pragma unroll
@@ -605,10 +627,9 @@ __global__ void __launch_bounds__(384, 1)
         float s[128];
 #pragma unroll
         for (int c = 0; c < 128; ++c) s[c] = __uint_as_float(sr[c / 32][c % 32]);
-        const int col0 = (w.tile0 + j) * kTileKeys;
-        const bool masked = col0 + kTileKeys - 1 > min(first_lim, w.len - 1);
-        if (masked) {
-          const int lim = min(lim_row, w.len - 1) - col0;
+        const int key0 = (w.tile0 + j) * kTileKeys;
+        if (key0 + kTileKeys - 1 > min(first_lim, w.len - 1)) {
+          const int lim = min(lim_row, w.len - 1) - key0;
 #pragma unroll
           for (int c = 0; c < 128; ++c) s[c] = c > lim ? -INFINITY : s[c];
         }
@@ -625,19 +646,16 @@ __global__ void __launch_bounds__(384, 1)
         mx1 = fmax3(mx1, s[126], s[127]);
         const float mx = fmax3(fmaxf(mx0, mx1), mx2, mx3) * scale_log2;
         const float cand = fmaxf(m, mx);
-        const bool update = (j == 0) || (cand > m + kRescaleThreshold);
+        const bool update = (j == j0) || (cand > m + kRescaleThreshold);
         const float m_new = update ? cand : m;
-        const bool rescale = (j > 0) && __any_sync(0xffffffffu, update);
+        const bool rescale = (j > j0) && __any_sync(0xffffffffu, update);
         const float alpha = rescale ? ((m_new == -INFINITY) ? 1.f : ex2_mufu(m - m_new)) : 1.f;
         m = m_new;
         const float mb = (m == -INFINITY) ? 0.f : m;
         const float rowsum = exp_pack_store<0, true>(s, scale_log2, mb, t_s);
         l = l * alpha + rowsum;
         if (rescale) {
-          if (QTiles == 1) {  // S runs two steps ahead: P V of the step before may still be at work on O
-            if (!warp_wait(bar(L::kOFull + 1), (pv_seen + j - 1) & 1u, ctl, kStatusTimeoutSoftmax)) { ok = false; break; }
-            tc_fence_after();
-          }
+          // O_i holds every earlier step of this stream: the commit that released S covers them
           const float2 a2 = make_float2(alpha, alpha);
 #pragma unroll 1
           for (int c = 0; c < 4; ++c) {
@@ -656,76 +674,110 @@ __global__ void __launch_bounds__(384, 1)
         tmem_st_wait();
         tc_fence_before();
         __syncwarp();
-        if (lane == 0) mbar_arrive(bar(L::kPFull + sb));
+        if (lane == 0) mbar_arrive(bar(L::kPFull + i));
       }
-      if (!ok) break;
-      pv_seen += ni;
       // ------------------------------ epilogue ------------------------------
-      uint32_t oall[4][32];
-      if (ni > 0) {
-        if (!warp_wait(bar(L::kOFull + i), o_full_par, ctl, kStatusTimeoutSoftmax)) { ok = false; break; }
-        o_full_par ^= 1u;
-        tc_fence_after();
+      float ov[kCols];
+      if constexpr (QTiles == 1) {
+        // both streams' (m, l), and whether every warp got here
+        ml_shared[i * 128 + row] = make_float2(m, l);
+        if (!pair_all(1, 256, ok)) { ok = false; break; }
+        const float2 x0 = ml_shared[row], x1 = ml_shared[128 + row];
+        named_sync(1, 256);  // both are read: the next piece may write
+        const float top = fmaxf(x0.x, x1.x), zero = top == -INFINITY ? 0.f : top;
+        const float a0 = exp2f(x0.x - zero), a1 = exp2f(x1.x - zero);
+        m = top;
+        l = x0.y * a0 + x1.y * a1;
 #pragma unroll
-        for (int c = 0; c < 4; ++c) tmem_ld32(t_o + c * 32, oall[c]);
-        tmem_ld_wait();
-        tc_fence_before();
-        __syncwarp();
-        if (lane == 0) mbar_arrive(bar(L::kOEmpty + i));
+        for (int c = 0; c < kCols; ++c) ov[c] = 0.f;
+#pragma unroll
+        for (int x = 0; x < 2; ++x) {
+          if (ni > x && ok) {
+            ok = warp_wait(bar(L::kOFull + x), (o_full_par >> x) & 1u, ctl, kStatusTimeoutSoftmax);
+            o_full_par ^= 1u << x;
+            if (ok) {
+              tc_fence_after();
+              uint32_t part[kCols / 32][32];
+#pragma unroll
+              for (int c = 0; c < kCols / 32; ++c) tmem_ld32(tmem + lane_off + 256 + x * 128 + col0 + c * 32, part[c]);
+              tmem_ld_wait();
+              tc_fence_before();
+              __syncwarp();
+              if (lane == 0) mbar_arrive(bar(L::kOEmpty + x));
+              const float a = x == 0 ? a0 : a1;
+#pragma unroll
+              for (int c = 0; c < kCols; ++c) ov[c] = fmaf(__uint_as_float(part[c / 32][c % 32]), a, ov[c]);
+            }
+          }
+        }
+        if (!ok) break;
       } else {
+        if (!ok) break;
+        if (ni > 0) {
+          if (!warp_wait(bar(L::kOFull + i), o_full_par, ctl, kStatusTimeoutSoftmax)) { ok = false; break; }
+          o_full_par ^= 1u;
+          tc_fence_after();
+          uint32_t part[4][32];
 #pragma unroll
-        for (int c = 0; c < 128; ++c) oall[c / 32][c % 32] = 0u;
+          for (int c = 0; c < 4; ++c) tmem_ld32(t_o + c * 32, part[c]);
+          tmem_ld_wait();
+          tc_fence_before();
+          __syncwarp();
+          if (lane == 0) mbar_arrive(bar(L::kOEmpty + i));
+#pragma unroll
+          for (int c = 0; c < kCols; ++c) ov[c] = __uint_as_float(part[c / 32][c % 32]);
+        } else {
+#pragma unroll
+          for (int c = 0; c < kCols; ++c) ov[c] = 0.f;
+        }
       }
-      auto ov = [&](int c) -> float { return __uint_as_float(oall[c / 32][c % 32]); };
+      if (!live) continue;
       if (w.cnt < w.n) {  // a piece: (m, l, O) to the workspace
-        const int64_t tile = part_tile(2 * blockIdx.x + (w.tile0 == 0 ? 1 : 0), QTiles, i);
-        float4* dst = reinterpret_cast<float4*>(p.part_o) + tile * 4096 + row;
-        if (live) {
+        const int64_t at = part_tile(2 * blockIdx.x + (w.tile0 == 0 ? 1 : 0), QTiles, tile);
+        float4* dst = reinterpret_cast<float4*>(p.part_o) + at * 4096 + (col0 / 4) * 128 + row;
 #pragma unroll
-          for (int c = 0; c < 32; ++c) dst[c * 128] = make_float4(ov(4 * c), ov(4 * c + 1), ov(4 * c + 2), ov(4 * c + 3));
-          reinterpret_cast<float2*>(p.part_ml)[tile * 128 + row] = make_float2(m, l);
-        }
-      } else if (live) {
-        const int64_t token = w.token0 + t0 + row_token;
-        const int head = w.h * p.group + row_head;
-        const int64_t orow = token * p.heads + head, lse_at = static_cast<int64_t>(head) * p.total_q + token;
-        float a = 1.f, x = 0.f;
-        if (p.add_o != nullptr) {  // the other result of this row, joined in
-          const float other = __ldcg(p.add_lse + lse_at) * 1.4426950408889634f;
-          const float top = fmaxf(m, other);
-          if (top != -INFINITY) {
-            a = exp2f(m - top);
-            x = exp2f(other - top);
-            l = l * a + x;
-            m = top;
-          }
-        }
-        const float inv = l == 0.f ? 0.f : 1.f / l;
-        a *= inv;
-        x *= inv;
-        const float4* add = reinterpret_cast<const float4*>(p.add_o + orow * 128);
-#pragma unroll
-        for (int c = 0; c < 32; c += 2) {
-          float4 u = make_float4(ov(4 * c) * a, ov(4 * c + 1) * a, ov(4 * c + 2) * a, ov(4 * c + 3) * a);
-          float4 v = make_float4(ov(4 * c + 4) * a, ov(4 * c + 5) * a, ov(4 * c + 6) * a, ov(4 * c + 7) * a);
-          if (p.add_o != nullptr) {
-            const float4 e = __ldcg(add + c), f = __ldcg(add + c + 1);
-            u = make_float4(fmaf(e.x, x, u.x), fmaf(e.y, x, u.y), fmaf(e.z, x, u.z), fmaf(e.w, x, u.w));
-            v = make_float4(fmaf(f.x, x, v.x), fmaf(f.y, x, v.y), fmaf(f.z, x, v.z), fmaf(f.w, x, v.w));
-          }
-          if (p.o != nullptr) {
-            *reinterpret_cast<uint4*>(p.o + orow * 128 + c * 4) =
-                make_uint4(pack_bf16x2(u.x, u.y), pack_bf16x2(u.z, u.w), pack_bf16x2(v.x, v.y), pack_bf16x2(v.z, v.w));
-          } else {
-            reinterpret_cast<float4*>(p.o32 + orow * 128)[c] = u;
-            reinterpret_cast<float4*>(p.o32 + orow * 128)[c + 1] = v;
-          }
-        }
-        if (p.lse != nullptr) p.lse[lse_at] = l == 0.f ? -INFINITY : m * kLn2 + logf(l);
+        for (int c = 0; c < kCols / 4; ++c)
+          dst[c * 128] = make_float4(ov[4 * c], ov[4 * c + 1], ov[4 * c + 2], ov[4 * c + 3]);
+        if (col0 == 0) reinterpret_cast<float2*>(p.part_ml)[at * 128 + row] = make_float2(m, l);
+        continue;
       }
+      const int64_t token = w.token0 + t0 + row_token;
+      const int head = w.h * p.group + row_head;
+      const int64_t orow = token * p.heads + head, lse_at = static_cast<int64_t>(head) * p.total_q + token;
+      float a = 1.f, x = 0.f;
+      if (p.add_o != nullptr) {  // the other result of this row, joined in
+        const float other = __ldcg(p.add_lse + lse_at) * 1.4426950408889634f;
+        const float top = fmaxf(m, other);
+        if (top != -INFINITY) {
+          a = exp2f(m - top);
+          x = exp2f(other - top);
+          l = l * a + x;
+          m = top;
+        }
+      }
+      const float inv = l == 0.f ? 0.f : 1.f / l;
+      a *= inv;
+      x *= inv;
+      const float4* add = reinterpret_cast<const float4*>(p.add_o + orow * 128 + col0);
+#pragma unroll
+      for (int c = 0; c < kCols / 4; c += 2) {
+        float4 u = make_float4(ov[4 * c] * a, ov[4 * c + 1] * a, ov[4 * c + 2] * a, ov[4 * c + 3] * a);
+        float4 v = make_float4(ov[4 * c + 4] * a, ov[4 * c + 5] * a, ov[4 * c + 6] * a, ov[4 * c + 7] * a);
+        if (p.add_o != nullptr) {
+          const float4 e = __ldcg(add + c), f = __ldcg(add + c + 1);
+          u = make_float4(fmaf(e.x, x, u.x), fmaf(e.y, x, u.y), fmaf(e.z, x, u.z), fmaf(e.w, x, u.w));
+          v = make_float4(fmaf(f.x, x, v.x), fmaf(f.y, x, v.y), fmaf(f.z, x, v.z), fmaf(f.w, x, v.w));
+        }
+        if (p.o != nullptr) {
+          *reinterpret_cast<uint4*>(p.o + orow * 128 + col0 + c * 4) =
+              make_uint4(pack_bf16x2(u.x, u.y), pack_bf16x2(u.z, u.w), pack_bf16x2(v.x, v.y), pack_bf16x2(v.z, v.w));
+        } else {
+          reinterpret_cast<float4*>(p.o32 + orow * 128 + col0)[c] = u;
+          reinterpret_cast<float4*>(p.o32 + orow * 128 + col0)[c + 1] = v;
+        }
+      }
+      if (p.lse != nullptr && col0 == 0) p.lse[lse_at] = l == 0.f ? -INFINITY : m * kLn2 + logf(l);
     }
-  } else {
-    regs_release<kOtherRegs>();  // warps 4-7 when QTiles == 1
   }
 
   tc_fence_before();
@@ -738,12 +790,13 @@ __global__ void __launch_bounds__(384, 1)
 
 // Adds up the pieces of the units that paged_tile_kernel cut, in key order: O = sum 2^(m_c - M) O_c / L,
 // M = max m_c, L = sum 2^(m_c - M) l_c. Reads each piece once and writes each row once: L2 traffic, and at
-// small sizes its latency. A work item is a unit's Q tile and C of its 32 column pieces, 128 rows wide, the
-// unit's pieces in two halves; C = 1 gives two units of 64 pieces enough items for every SM, C = 4 keeps
-// more loads in flight where there are many units of few pieces.
-template <int QTiles, int C>
+// small sizes its latency. 128 threads take C of the 32 column pieces of a unit's Q tile, one row each.
+// Halves = 1: the two halves of a block work on their own (many units, few pieces each). Halves = 2: they
+// share one item's pieces (two units of 64 pieces still have work for every SM).
+template <int QTiles, int C, int Halves>
 __device__ __forceinline__ void join_items(const PagedTileParams& tp, const int4* cuts, const int* first_block,
-                                           int count, float4 (*half_o)[128], float2* half_ml) {
+                                           int count, float4* half_o, float2* half_ml) {
+  static_assert(Halves == 1 || C == 1, "the halves meet in one piece per row");
   constexpr int kBatch = 8 / C;  // pieces whose loads are in flight together
   const PagedParams& p = tp.p;
   const int row = threadIdx.x % 128, half = threadIdx.x / 128;
@@ -751,70 +804,68 @@ __device__ __forceinline__ void join_items(const PagedTileParams& tp, const int4
   const float4* part_o = reinterpret_cast<const float4*>(p.part_o);
   const float2* part_ml = reinterpret_cast<const float2*>(p.part_ml);
   const int items = count * QTiles * (32 / C);
-  for (int item = blockIdx.x; item < items; item += gridDim.x) {
+  const int first = Halves == 1 ? blockIdx.x * 2 + half : blockIdx.x, stride = Halves == 1 ? gridDim.x * 2 : gridDim.x;
+  for (int item = first; item < items; item += stride) {
     const int u = item / (QTiles * (32 / C)), i = item / (32 / C) % QTiles, col = item % (32 / C) * C;
     const int4 c = cuts[u];
     const int t0 = i * tp.tile_tokens;
-    if (t0 >= c.y) continue;  // block-uniform
+    if (t0 >= c.y) continue;  // the same for all threads that share the item
     const bool live = row_token < tp.tile_tokens && t0 + row_token < c.y;
-    const int c0 = first_block[u], parts = c.w - c0 + 1;
-    const int mid = (parts + 1) / 2, from = half ? mid : 0, to = half ? parts : mid;
+    if (Halves == 1 && !live) continue;
+    const int64_t token = c.x + t0 + row_token;
+    const int head = c.z * p.group + row_head;
+    const int64_t orow = token * p.heads + head, lse_at = static_cast<int64_t>(head) * p.total_q + token;
+    const int c0 = first_block[u], parts = c.w - c0 + 1, mid = (parts + 1) / 2;
+    const int from = Halves == 2 && half ? mid : 0, to = Halves == 2 && !half ? mid : parts;
     auto tile = [&](int x) { return part_tile(2 * (c0 + x) + (x == 0 ? 1 : 0), QTiles, i); };
     float m = -INFINITY, l = 0.f;
     float4 acc[C];
 #pragma unroll
     for (int e = 0; e < C; ++e) acc[e] = make_float4(0.f, 0.f, 0.f, 0.f);
-    if (live) {
-      for (int x0 = from; x0 < to; x0 += kBatch) {
-        float2 ml[kBatch];
-        float4 o[kBatch][C];
+    for (int x0 = from; x0 < to && live; x0 += kBatch) {
+      float2 ml[kBatch];
+      float4 o[kBatch][C];
 #pragma unroll
-        for (int x = 0; x < kBatch; ++x) {
-          if (x0 + x < to) {
-            ml[x] = __ldcg(part_ml + tile(x0 + x) * 128 + row);
+      for (int x = 0; x < kBatch; ++x) {
+        ml[x] = make_float2(-INFINITY, 0.f);
+        if (x0 + x < to) ml[x] = __ldcg(part_ml + tile(x0 + x) * 128 + row);
 #pragma unroll
-            for (int e = 0; e < C; ++e) o[x][e] = __ldcg(part_o + tile(x0 + x) * 4096 + (col + e) * 128 + row);
-          } else {
-            ml[x] = make_float2(-INFINITY, 0.f);
-#pragma unroll
-            for (int e = 0; e < C; ++e) o[x][e] = make_float4(0.f, 0.f, 0.f, 0.f);
-          }
-        }
-        float top = m;
-#pragma unroll
-        for (int x = 0; x < kBatch; ++x) top = fmaxf(top, ml[x].x);
-        // relative to 0 while no piece has seen a key: NaN sums still go through
-        const float zero = top == -INFINITY ? 0.f : top, a = exp2f(m - zero);
-        l *= a;
-        m = top;
-#pragma unroll
-        for (int e = 0; e < C; ++e) acc[e] = make_float4(acc[e].x * a, acc[e].y * a, acc[e].z * a, acc[e].w * a);
-#pragma unroll
-        for (int x = 0; x < kBatch; ++x) {
-          const float b = exp2f(ml[x].x - zero);
-          l = fmaf(ml[x].y, b, l);
-#pragma unroll
-          for (int e = 0; e < C; ++e)
-            acc[e] = make_float4(fmaf(o[x][e].x, b, acc[e].x), fmaf(o[x][e].y, b, acc[e].y),
-                                 fmaf(o[x][e].z, b, acc[e].z), fmaf(o[x][e].w, b, acc[e].w));
+        for (int e = 0; e < C; ++e) {
+          o[x][e] = make_float4(0.f, 0.f, 0.f, 0.f);
+          if (x0 + x < to) o[x][e] = __ldcg(part_o + tile(x0 + x) * 4096 + (col + e) * 128 + row);
         }
       }
-    }
-    if (half) {
+      float top = m;
 #pragma unroll
-      for (int e = 0; e < C; ++e) half_o[e][row] = acc[e];
-      half_ml[row] = make_float2(m, l);
+      for (int x = 0; x < kBatch; ++x) top = fmaxf(top, ml[x].x);
+      // relative to 0 while no piece has seen a key: NaN sums still go through
+      const float zero = top == -INFINITY ? 0.f : top, a = exp2f(m - zero);
+      l *= a;
+      m = top;
+#pragma unroll
+      for (int e = 0; e < C; ++e) acc[e] = make_float4(acc[e].x * a, acc[e].y * a, acc[e].z * a, acc[e].w * a);
+#pragma unroll
+      for (int x = 0; x < kBatch; ++x) {
+        const float b = exp2f(ml[x].x - zero);
+        l = fmaf(ml[x].y, b, l);
+#pragma unroll
+        for (int e = 0; e < C; ++e)
+          acc[e] = make_float4(fmaf(o[x][e].x, b, acc[e].x), fmaf(o[x][e].y, b, acc[e].y),
+                               fmaf(o[x][e].z, b, acc[e].z), fmaf(o[x][e].w, b, acc[e].w));
+      }
     }
-    __syncthreads();
-    if (!half && live) {
-      const int64_t token = c.x + t0 + row_token;
-      const int head = c.z * p.group + row_head;
-      const int64_t orow = token * p.heads + head, lse_at = static_cast<int64_t>(head) * p.total_q + token;
-      const float2 ml = half_ml[row];
+    if (Halves == 2) {
+      if (half) {
+        half_o[row] = acc[0];
+        half_ml[row] = make_float2(m, l);
+      }
+      __syncthreads();
+    }
+    if (live && (Halves == 1 || !half)) {
+      const float2 ml = Halves == 2 ? half_ml[row] : make_float2(-INFINITY, 0.f);
       const float other = p.add_o != nullptr ? __ldcg(p.add_lse + lse_at) * 1.4426950408889634f : -INFINITY;
-      const float top = fmax3(m, ml.x, other);
-      const bool any = top != -INFINITY;
-      float a = any ? exp2f(m - top) : 0.f, b = any ? exp2f(ml.x - top) : 0.f, x = any ? exp2f(other - top) : 0.f;
+      const float top = fmax3(m, ml.x, other), zero = top == -INFINITY ? 0.f : top;
+      float a = exp2f(m - zero), b = exp2f(ml.x - zero), x = exp2f(other - zero);
       l = l * a + ml.y * b + x;
       const float inv = l == 0.f ? 0.f : 1.f / l;
       a *= inv;
@@ -822,8 +873,11 @@ __device__ __forceinline__ void join_items(const PagedTileParams& tp, const int4
       x *= inv;
 #pragma unroll
       for (int e = 0; e < C; ++e) {
-        const float4 o = half_o[e][row];
-        float4 v = make_float4(acc[e].x * a + o.x * b, acc[e].y * a + o.y * b, acc[e].z * a + o.z * b, acc[e].w * a + o.w * b);
+        float4 v = make_float4(acc[e].x * a, acc[e].y * a, acc[e].z * a, acc[e].w * a);
+        if (Halves == 2) {
+          const float4 o = half_o[row];
+          v = make_float4(fmaf(o.x, b, v.x), fmaf(o.y, b, v.y), fmaf(o.z, b, v.z), fmaf(o.w, b, v.w));
+        }
         if (p.add_o != nullptr) {
           const float4 f = __ldcg(reinterpret_cast<const float4*>(p.add_o + orow * 128) + col + e);
           v = make_float4(fmaf(f.x, x, v.x), fmaf(f.y, x, v.y), fmaf(f.z, x, v.z), fmaf(f.w, x, v.w));
@@ -836,7 +890,7 @@ __device__ __forceinline__ void join_items(const PagedTileParams& tp, const int4
       }
       if (p.lse != nullptr && col == 0) p.lse[lse_at] = l == 0.f ? -INFINITY : top * kLn2 + logf(l);
     }
-    __syncthreads();
+    if (Halves == 2) __syncthreads();
   }
 }
 
@@ -848,7 +902,7 @@ __global__ void __launch_bounds__(256, kJoinPerSm) paged_join_kernel(const __gri
   __shared__ int4 cuts[kMaxCuts];
   __shared__ int first_block[kMaxCuts];
   __shared__ int warp_cuts[kMaxCuts / 32];
-  __shared__ float4 half_o[4][128];
+  __shared__ float4 half_o[128];
   __shared__ float2 half_ml[128];
   wait_for_predecessor();
   // the cut units, numbered alike in every block: by the block that opens them (blocks <= kMaxCuts threads)
@@ -869,9 +923,9 @@ __global__ void __launch_bounds__(256, kJoinPerSm) paged_join_kernel(const __gri
   }
   __syncthreads();
   if (count * QTiles * 32 > 2 * static_cast<int>(gridDim.x))
-    join_items<QTiles, 4>(tp, cuts, first_block, count, half_o, half_ml);
+    join_items<QTiles, 4, 1>(tp, cuts, first_block, count, half_o, half_ml);
   else
-    join_items<QTiles, 1>(tp, cuts, first_block, count, half_o, half_ml);
+    join_items<QTiles, 1, 2>(tp, cuts, first_block, count, half_o, half_ml);
 }
 
 }  // namespace fav4
