@@ -79,17 +79,36 @@ struct AppendParams {
   int heads, total_q, rotary, table_rows;
 };
 
-// The sequence of packed row t: the number of b with cu[b+1] <= t. 32 probes per step.
-__device__ __forceinline__ int find_sequence(const int* cu, int batch, int t, int lane) {
-  int lo = 0, hi = batch;
-  while (lo < hi) {
+// The sequence of packed row t, i.e. the number of b with cu[b+1] <= t, by 32 probes a step; the last step
+// brings what the caller needs of the sequence along, so that a warp waits once less. False: t belongs to no
+// sequence.
+struct AppendSeq {
+  int b, begin, end, len, offset;
+};
+__device__ __forceinline__ bool find_sequence(const PagedCacheView& c, const int* cu, const int* offsets, int t,
+                                              int lane, AppendSeq* out) {
+  int lo = 0, hi = c.batch;  // the answer is in [lo, hi]
+  while (hi - lo > 31) {
     const int step = (hi - lo + 31) / 32;
     const int64_t i = lo + static_cast<int64_t>(lane) * step + step - 1;
     const bool before = i < hi && __ldg(cu + i + 1) <= t;
     lo += __popc(__ballot_sync(0xffffffffu, before)) * step;
     hi = min(hi, lo + step - 1);
   }
-  return lo;
+  const int i = lo + lane;
+  const bool any = i < c.batch;
+  AppendSeq s;
+  s.begin = any ? __ldg(cu + i) : 0;
+  s.end = any ? __ldg(cu + i + 1) : 0;
+  s.len = any ? __ldg(c.lens + i) : 0;
+  s.offset = any && offsets != nullptr ? __ldg(offsets + i) : 0;
+  const int at = __popc(__ballot_sync(0xffffffffu, i < hi && s.end <= t));
+  out->b = lo + at;
+  out->begin = __shfl_sync(0xffffffffu, s.begin, at);
+  out->end = __shfl_sync(0xffffffffu, s.end, at);
+  out->len = __shfl_sync(0xffffffffu, s.len, at);
+  out->offset = __shfl_sync(0xffffffffu, s.offset, at);
+  return out->b < c.batch && out->begin <= t && t < out->end;  // offsets out of order: no sequence
 }
 
 __device__ __forceinline__ void rotate_pairs(uint32_t& a, uint32_t& b, float2 c, float2 s) {
@@ -140,14 +159,12 @@ __global__ void __launch_bounds__(256) paged_append_kernel(const __grid_constant
       b[u] = *reinterpret_cast<const uint4*>(src + pb * 8);
     }
   }
-  const int seq = find_sequence(p.cu, p.c.batch, t, lane);
-  if (seq >= p.c.batch) return;  // a row of no sequence
-  const int qa = __ldg(p.cu + seq), qe = __ldg(p.cu + seq + 1);
-  if (t < qa || t >= qe) return;  // offsets out of order
-  const int64_t pos = static_cast<int64_t>(__ldg(p.c.lens + seq)) - qe + t;
+  AppendSeq seq;
+  if (!find_sequence(p.c, p.cu, p.offsets, t, lane, &seq)) return;
+  const int64_t pos = static_cast<int64_t>(seq.len) - seq.end + t;
   float4 cs[2], sn[2];
   if (turned) {
-    const int64_t at = pos + (p.offsets != nullptr ? __ldg(p.offsets + seq) : 0);
+    const int64_t at = pos + seq.offset;
     const int64_t row = min(max(at, int64_t(0)), static_cast<int64_t>(p.table_rows) - 1);
     const float4* cp = reinterpret_cast<const float4*>(p.cos_t + row * (p.rotary / 2) + slot * 8);
     const float4* sp = reinterpret_cast<const float4*>(p.sin_t + row * (p.rotary / 2) + slot * 8);
@@ -159,7 +176,7 @@ __global__ void __launch_bounds__(256) paged_append_kernel(const __grid_constant
   int64_t dst_kv = -1;  // a position without a slot (negative, past the table, no such page) is not written
   if (r0 + kAppendRows > p.heads && pos >= 0 && pos < static_cast<int64_t>(p.c.max_pages) * p.c.page_size) {
     const int idx = static_cast<int>(pos) / p.c.page_size;
-    const int page = __ldg(p.c.table + seq * p.c.table_stride + idx);
+    const int page = __ldg(p.c.table + seq.b * p.c.table_stride + idx);
     if (page >= 0 && page < p.c.num_pages)
       dst_kv = page * p.c.page_stride + (static_cast<int>(pos) - idx * p.c.page_size) * p.c.token_stride;
   }
@@ -247,6 +264,11 @@ constexpr int kPagedList = 64;   // pieces that are listed at a time
 constexpr int kPagedSmem = kPagedWarps * kPagedRing;
 static_assert(kPagedRows * 128 * 4 <= kPagedStageBytes, "a warp's O is left in one ring slot");
 
+__device__ __forceinline__ uint32_t add_acq_rel(uint32_t* p) {
+  uint32_t old;
+  asm volatile("atom.acq_rel.gpu.global.add.u32 %0, [%1], 1;" : "=r"(old) : "l"(p) : "memory");
+  return old;
+}
 __device__ __forceinline__ void cp_async16(uint32_t dst, const void* src, int bytes) {
   asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(bytes) : "memory");
 }
@@ -658,10 +680,10 @@ __global__ void __launch_bounds__(kPagedWarps * 32, 2) paged_attn_kernel(const _
         }
       }
       if (!whole) {
-        __threadfence();
         __syncthreads();
         if (tid == 0) {
-          const uint32_t before = atomicAdd(p.arrived + w.c0, 1u);
+          // after the barrier, this thread's release and acquire stand for the whole block's
+          const uint32_t before = add_acq_rel(p.arrived + w.c0);
           last_one = before == static_cast<uint32_t>(w.c1 - w.c0);
           if (last_one) p.arrived[w.c0] = 0u;  // ready for the next launch
         }
@@ -669,7 +691,6 @@ __global__ void __launch_bounds__(kPagedWarps * 32, 2) paged_attn_kernel(const _
         if (last_one) {
           // this block is the last of the unit's: it adds the pieces up in the order of their keys. With fewer
           // rows than warps, the warps share a row's pieces.
-          __threadfence();
           const int share = rows == 1 ? 4 : rows == 2 ? 2 : 1;
           const int turn = warp % share, parts = w.c1 - w.c0 + 1;
           const int x_begin = parts * turn / share, x_end = parts * (turn + 1) / share;
