@@ -36,10 +36,12 @@ struct SeqView {
 };
 
 // a / b for a >= 0, b > 0. Work counts are 64-bit, but nearly always small: a 64-bit division costs several
-// times a 32-bit one, and the schedules wait for theirs.
+// times a 32-bit one, and the schedules wait for theirs. The long way is kept out of line: code that a kernel
+// fetches once, at its start, costs it more than the arithmetic.
+__host__ __device__ __noinline__ inline int64_t divide64(int64_t a, int64_t b) { return a / b; }
 __host__ __device__ __forceinline__ int64_t quotient(int64_t a, int64_t b) {
   if (((a | b) >> 32) == 0) return static_cast<uint32_t>(a) / static_cast<uint32_t>(b);
-  return a / b;
+  return divide64(a, b);
 }
 
 __device__ __forceinline__ SeqView seq_view(const PagedCacheView& c, const int* cu, int total_q, int max_sq, int b) {
@@ -320,7 +322,7 @@ __device__ __forceinline__ bool row_place(const PagedParams& p, const SeqView& s
 }
 
 // One finished row: columns 4 lane .. 4 lane + 3 of sum / l, joined with the other result if there is one.
-__device__ __forceinline__ void finish_row(const PagedParams& p, const RowPlace& at, float4 acc, float m, float l,
+__device__ __noinline__ void finish_row(const PagedParams& p, const RowPlace& at, float4 acc, float m, float l,
                                            int lane) {
   const int64_t row = static_cast<int64_t>(at.token) * p.heads + at.head;
   const int64_t lse_at = static_cast<int64_t>(at.head) * p.total_q + at.token;
@@ -524,7 +526,7 @@ __global__ void __launch_bounds__(kPagedWarps * 32, 2) paged_attn_kernel(const _
       cp_async_commit();
       slot_in = slot_in == kPagedStages - 1 ? 0 : slot_in + 1;
     };
-#pragma unroll
+#pragma unroll 1
     for (int i = 0; i < kPagedStages - 1; ++i) issue();
 
     uint32_t qf[8][4];
@@ -698,11 +700,11 @@ __global__ void __launch_bounds__(kPagedWarps * 32, 2) paged_attn_kernel(const _
             auto part_row = [&](int x) { return static_cast<int64_t>(2 * (w.c0 + x) + (x == 0 ? 1 : 0)) * kPagedRows + r; };
             float top = -INFINITY, sum = 0.f;
             float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
-            for (int x0 = x_begin; x0 < x_end; x0 += 12) {
-              float4 v[12];
-              float2 ml[12];
+            for (int x0 = x_begin; x0 < x_end; x0 += 8) {
+              float4 v[8];
+              float2 ml[8];
 #pragma unroll
-              for (int x = 0; x < 12; ++x) {
+              for (int x = 0; x < 8; ++x) {
                 ml[x] = make_float2(-INFINITY, 0.f);
                 v[x] = make_float4(0.f, 0.f, 0.f, 0.f);
                 if (x0 + x < x_end) {
@@ -712,14 +714,14 @@ __global__ void __launch_bounds__(kPagedWarps * 32, 2) paged_attn_kernel(const _
               }
               float next = top;
 #pragma unroll
-              for (int x = 0; x < 12; ++x) next = fmaxf(next, ml[x].x);
+              for (int x = 0; x < 8; ++x) next = fmaxf(next, ml[x].x);
               // relative to 0 while no piece has seen a key: NaN sums still go through
               const float zero = next == -INFINITY ? 0.f : next, a = exp2f(top - zero);
               acc = make_float4(acc.x * a, acc.y * a, acc.z * a, acc.w * a);
               sum *= a;
               top = next;
 #pragma unroll
-              for (int x = 0; x < 12; ++x) {
+              for (int x = 0; x < 8; ++x) {
                 const float c = exp2f(ml[x].x - zero);
                 acc = make_float4(acc.x + c * v[x].x, acc.y + c * v[x].y, acc.z + c * v[x].z, acc.w + c * v[x].w);
                 sum += c * ml[x].y;

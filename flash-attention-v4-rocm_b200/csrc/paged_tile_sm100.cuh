@@ -44,6 +44,19 @@ struct PagedTileParams {
   uint64_t wait_limit_ns;
 };
 
+// The waits of sm100.cuh with the part that does wait out of line, for the warps that can afford the call: a
+// kernel of a few microseconds notices the code that it fetches. The MMA and softmax warps, whose waits are
+// on the way of every step, keep theirs in line (out of line in the MMA warp: 2 % slower on long chunks).
+__device__ __noinline__ bool wait_long(uint32_t bar, uint32_t parity, WaitCtl ctl, uint32_t code) {
+  return mbar_wait(bar, parity, ctl, code);
+}
+__device__ __forceinline__ bool wait_phase(uint32_t bar, uint32_t parity, const WaitCtl& ctl, uint32_t code) {
+  return mbar_test(bar, parity) || wait_long(bar, parity, ctl, code);
+}
+__device__ __forceinline__ bool warp_wait_phase(uint32_t bar, uint32_t parity, const WaitCtl& ctl, uint32_t code) {
+  return __all_sync(0xffffffffu, wait_phase(bar, parity, ctl, code));
+}
+
 // A stretch of one unit.
 struct Piece {
   int token0, tokens;   // the unit's first row of Q, and how many tokens it has
@@ -56,7 +69,7 @@ static_assert(sizeof(Piece) == 64, "four 16-byte words");
 
 // sum over j < n of floor((a j + c) / 128), for a, c >= 0, by the steps of Euclid's algorithm. Blocks wait
 // for it, so the first step (by 128) has no division and the others one each: their c and a are below 128.
-__host__ __device__ __forceinline__ int64_t floor_sum128(int64_t n, int64_t a, int64_t c) {
+__host__ __device__ __noinline__ inline int64_t floor_sum128(int64_t n, int64_t a, int64_t c) {
   if (n <= 0) return 0;
   int64_t s = n * (n - 1) / 2 * (a >> 7) + n * (c >> 7);
   int m = 128, r = static_cast<int>(a & 127), d = static_cast<int>(c & 127);
@@ -86,7 +99,7 @@ __host__ __device__ __forceinline__ int unit_steps(const SeqView& s, int causal,
   const int64_t last = full < s.sq ? full : s.sq;
   return steps_up_to(causal ? static_cast<int64_t>(s.len) - s.sq + last : s.len);
 }
-__host__ __device__ __forceinline__ int64_t units_steps(const SeqView& s, int causal, int bt, int64_t r) {
+__host__ __device__ __noinline__ inline int64_t units_steps(const SeqView& s, int causal, int bt, int64_t r) {
   if (r <= 0) return 0;
   if (!causal) return r * steps_up_to(s.len);
   const int64_t units = quotient(static_cast<int64_t>(s.sq) + bt - 1, bt);
@@ -243,9 +256,10 @@ __global__ void __launch_bounds__(384, 1)
 
   // Reads the next piece; every warp that calls it does so converged and releases the slot at once.
   int piece_at = 0;
-  auto next_piece = [&](Piece* out) -> bool {
+  auto next_piece = [&](Piece* out, bool in_line = false) -> bool {
     const int s = piece_at % kPieceSlots;
-    if (!warp_wait(bar(L::kPieceFull + s), (piece_at / kPieceSlots) & 1u, ctl, kStatusTimeoutLoad)) return false;
+    if (in_line ? !warp_wait(bar(L::kPieceFull + s), (piece_at / kPieceSlots) & 1u, ctl, kStatusTimeoutLoad)
+                : !warp_wait_phase(bar(L::kPieceFull + s), (piece_at / kPieceSlots) & 1u, ctl, kStatusTimeoutLoad)) return false;
     const int4* src = reinterpret_cast<const int4*>(pieces + s);
     int4 w0 = src[0], w1 = src[1], w2 = src[2];
     out->token0 = w0.x; out->tokens = w0.y; out->past = w0.z; out->len = w0.w;
@@ -285,7 +299,7 @@ __global__ void __launch_bounds__(384, 1)
         const int n0 = tile_steps(w, 0), n1 = QTiles > 1 ? tile_steps(w, 1) : 0;
         const int N = max(n0, n1);
         if (N == 0) continue;
-        if (!warp_wait(bar(L::kQEmpty), st.q_empty(), ctl, kStatusTimeoutLoad)) { ok = false; break; }
+        if (!warp_wait_phase(bar(L::kQEmpty), st.q_empty(), ctl, kStatusTimeoutLoad)) { ok = false; break; }
         st.flip_q_empty();
         if (lane == 0) {
           mbar_arrive_expect_tx(bar(L::kQFull), ((n0 > 0 ? 1 : 0) + (n1 > 0 ? 1 : 0)) * 2 * q_box);
@@ -314,7 +328,7 @@ __global__ void __launch_bounds__(384, 1)
           const int j = g + lead;
           const int page_next = g + 1 + lead >= 0 ? page_of(g + 1 + lead) : 0;
           if (KA > 1 && !has_v && !has_k) { page = page_next; continue; }
-          if (!warp_wait(bar(L::kKVEmpty + ring.stage), ring.phase ^ 1u, ctl, kStatusTimeoutLoad)) { ok = false; break; }
+          if (!warp_wait_phase(bar(L::kKVEmpty + ring.stage), ring.phase ^ 1u, ctl, kStatusTimeoutLoad)) { ok = false; break; }
           const uint32_t fb = bar(L::kKVFull + ring.stage);
           auto tile_bytes = [&](int t) -> uint32_t {  // whole groups up to the last key
             const int64_t left = static_cast<int64_t>(w.len) - static_cast<int64_t>(w.tile0 + t) * kTileKeys;
@@ -342,7 +356,7 @@ __global__ void __launch_bounds__(384, 1)
         volatile uint32_t no_abort = 0;
         WaitCtl drain{&no_abort, tp.status, tp.wait_limit_ns};
         for (int s = 0; s < Slots; ++s)
-          if (st.was_armed(s)) mbar_wait(bar(L::kKVFull + s), st.armed_parity(s), drain, kStatusTimeoutDrain);
+          if (st.was_armed(s)) wait_phase(bar(L::kKVFull + s), st.armed_parity(s), drain, kStatusTimeoutDrain);
       }
       __syncwarp();
     } else if (warp == 9) {
@@ -487,7 +501,7 @@ __global__ void __launch_bounds__(384, 1)
         const int64_t first = static_cast<int64_t>(w.tile0 + N - 1) * kTileKeys;  // of the last V tile
         const int row = first + kTileKeys > w.len ? static_cast<int>(w.len - first) : kTileKeys;
         for (int left = N + min(KA, N); left > 0; --left) {
-          if (!warp_wait(bar(L::kKVFull + ring.stage), ring.phase, ctl, kStatusTimeoutLoad)) { ok = false; break; }
+          if (!warp_wait_phase(bar(L::kKVFull + ring.stage), ring.phase, ctl, kStatusTimeoutLoad)) { ok = false; break; }
           if (left == 1 && row < kTileKeys) {
             uint8_t* v = smem + L::kKV + ring.stage * L::kSlotBytes;
             for (int x = row * 8 + lane; x < kTileKeys * 8; x += 32) {
@@ -509,7 +523,7 @@ __global__ void __launch_bounds__(384, 1)
       bool ok = true;
       auto put = [&](const Piece& w) {  // lane 0
         const int s = out % kPieceSlots;
-        if (!mbar_wait(bar(L::kPieceEmpty + s), ((out / kPieceSlots) & 1u) ^ 1u, ctl, kStatusTimeoutLoad)) {
+        if (!wait_phase(bar(L::kPieceEmpty + s), ((out / kPieceSlots) & 1u) ^ 1u, ctl, kStatusTimeoutLoad)) {
           ok = false;
           return;
         }
@@ -607,7 +621,7 @@ __global__ void __launch_bounds__(384, 1)
     const int row_head = row - row_token * p.group;
     bool ok = true;
     Piece w;
-    while (ok && next_piece(&w)) {
+    while (ok && next_piece(&w, true)) {
       const int t0 = tile * tp.tile_tokens;
       if (t0 >= w.tokens) continue;  // no rows in this Q tile
       const int ni = tile_steps(w, tile);
