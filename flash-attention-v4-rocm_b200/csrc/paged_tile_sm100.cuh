@@ -317,7 +317,7 @@ __global__ void __launch_bounds__(384, 1)
         const int* table = p.c.table + w.b * p.c.table_stride;
         const int grp = lane % 16;
         auto page_of = [&](int j) -> int {
-          const int64_t key = static_cast<int64_t>(w.tile0 + j) * kTileKeys + grp * R;
+          const int key = (w.tile0 + j) * kTileKeys + grp * R;  // lengths stay 1024 below INT_MAX
           if (grp >= groups || j >= N || key >= w.len) return 0;
           return min(max(__ldg(table + key / p.c.page_size), 0), p.c.num_pages - 1);
         };
@@ -331,18 +331,18 @@ __global__ void __launch_bounds__(384, 1)
           if (!warp_wait_phase(bar(L::kKVEmpty + ring.stage), ring.phase ^ 1u, ctl, kStatusTimeoutLoad)) { ok = false; break; }
           const uint32_t fb = bar(L::kKVFull + ring.stage);
           auto tile_bytes = [&](int t) -> uint32_t {  // whole groups up to the last key
-            const int64_t left = static_cast<int64_t>(w.len) - static_cast<int64_t>(w.tile0 + t) * kTileKeys;
-            return left >= kTileKeys ? kTileBytes : static_cast<uint32_t>((left + R - 1) / R * R) * 256u;
+            const int left = w.len - (w.tile0 + t) * kTileKeys;
+            return left >= kTileKeys ? kTileBytes : static_cast<uint32_t>((left + R - 1) & -R) * 256u;
           };
           if (lane == 0)
             mbar_arrive_expect_tx(fb, (has_v ? tile_bytes(g) : 0u) + (has_k ? tile_bytes(g + KA) : 0u));
           st.arm(ring.stage, ring.phase);
           __syncwarp();
-          const int64_t key = static_cast<int64_t>(w.tile0 + j) * kTileKeys + grp * R;
+          const int key = (w.tile0 + j) * kTileKeys + grp * R;
           if (grp < groups && j >= 0 && j < N && key < w.len) {
             const uint32_t dst = sbase + L::kKV + ring.stage * L::kSlotBytes + (lane < 16 ? kTileBytes : 0) + grp * R * 128;
             const CUtensorMap* map = lane < 16 ? &tm_k : &tm_v;
-            const int slot = static_cast<int>(key % p.c.page_size);
+            const int slot = key % p.c.page_size;
             tma_load_4d(dst, map, fb, 0, w.h, slot, page, pol_kv);
             tma_load_4d(dst + kBoxBytes, map, fb, 64, w.h, slot, page, pol_kv);
           }
