@@ -11,11 +11,9 @@
 //
 //   warps 0-3 / 4-7  softmax, correction and epilogue, one row per thread: of Q tile 0 / 1, or of the even /
 //                    odd steps of the only Q tile
-//   warp 8           TMA: Q tiles, then the K/V ring; the lanes hold the page numbers of a tile's groups of
-//                    box_rows keys (a power of two that divides the page size) and each issues its own boxes
+//   warps 8 and 10   TMA: Q tiles and K, and V; the lanes hold the page numbers of a tile's groups of box_rows
+//                    keys (a power of two that divides the page size) and each issues its own boxes
 //   warp 9           one thread issues every tcgen05.mma
-//   warp 10          zeroes the V rows past the end of a sequence: those slots may hold NaN, and 0 * NaN in
-//                    P V would reach the result (their scores are masked, so K needs nothing)
 //   warp 11          the schedule: pieces of work into a small ring that the other warps read
 //
 // Schedule. A unit is (sequence, K/V head, Q tiles of `block_tokens` tokens) and has as many steps as
@@ -173,8 +171,8 @@ __global__ void __launch_bounds__(384, 1)
     mbar_init(bar(L::kQFull), 1);
     mbar_init(bar(L::kQEmpty), 1);
     for (int s = 0; s < Slots; ++s) {
-      mbar_init(bar(L::kKVFull + s), 1);
-      mbar_init(bar(L::kKVEmpty + s), 2);  // the MMAs that read it, and warp 10
+      mbar_init(bar(L::kKVFull + s), 2);  // the K side and the V side
+      mbar_init(bar(L::kKVEmpty + s), 1);
       mbar_init(bar(L::kVFix + s), 1);
     }
     for (int i = 0; i < 2; ++i) {
@@ -285,8 +283,14 @@ __global__ void __launch_bounds__(384, 1)
 
   if (warp >= 8) {
     regs_release<kTileOtherRegs>();
-    if (warp == 8) {
-      // ============================ TMA producer ============================
+    if (warp == 8 || warp == 10) {
+      // ============================ TMA producers ===========================
+      // Warp 8 loads Q and K, warp 10 loads V: issuing a box costs some tens of ns, and a tile of small pages has
+      // sixteen. The ring's groups are {K_0}, .., {V_g, K_(g+KA)}, .., {V_(N-1)}; both warps arrive at each. Warp 10
+      // then zeroes the V rows past the end of a sequence.
+      const bool side_v = warp == 10;
+      const CUtensorMap* map = side_v ? &tm_v : &tm_k;
+      const int lead = side_v ? 0 : KA;  // the tile of group g: g + lead
       const uint64_t pol_kv = policy_evict_last();
       const uint64_t pol_q = policy_evict_first();
       Ring ring;
@@ -299,55 +303,63 @@ __global__ void __launch_bounds__(384, 1)
         const int n0 = tile_steps(w, 0), n1 = QTiles > 1 ? tile_steps(w, 1) : 0;
         const int N = max(n0, n1);
         if (N == 0) continue;
-        if (!warp_wait_phase(bar(L::kQEmpty), st.q_empty(), ctl, kStatusTimeoutLoad)) { ok = false; break; }
-        st.flip_q_empty();
-        if (lane == 0) {
-          mbar_arrive_expect_tx(bar(L::kQFull), ((n0 > 0 ? 1 : 0) + (n1 > 0 ? 1 : 0)) * 2 * q_box);
-          for (int i = 0; i < QTiles; ++i) {
-            if ((i == 0 ? n0 : n1) == 0) continue;
-            const uint32_t dst = sbase + L::kQ + i * kTileBytes;
-            const int row = w.token0 + i * tp.tile_tokens;
-            tma_load_3d(dst, &tm_q, bar(L::kQFull), 0, w.h * p.group, row, pol_q);
-            tma_load_3d(dst + kBoxBytes, &tm_q, bar(L::kQFull), 64, w.h * p.group, row, pol_q);
+        if (!side_v) {
+          if (!warp_wait_phase(bar(L::kQEmpty), st.q_empty(), ctl, kStatusTimeoutLoad)) { ok = false; break; }
+          st.flip_q_empty();
+          if (lane == 0) {
+            mbar_arrive_expect_tx(bar(L::kQFull), ((n0 > 0 ? 1 : 0) + (n1 > 0 ? 1 : 0)) * 2 * q_box);
+            for (int i = 0; i < QTiles; ++i) {
+              if ((i == 0 ? n0 : n1) == 0) continue;
+              const uint32_t dst = sbase + L::kQ + i * kTileBytes;
+              const int row = w.token0 + i * tp.tile_tokens;
+              tma_load_3d(dst, &tm_q, bar(L::kQFull), 0, w.h * p.group, row, pol_q);
+              tma_load_3d(dst + kBoxBytes, &tm_q, bar(L::kQFull), 64, w.h * p.group, row, pol_q);
+            }
           }
+          __syncwarp();
         }
-        __syncwarp();
-        // Lane g < groups has the page of keys [128 t + g R, + R) of the K tile to come; lane 16 + g the same of
-        // the V tile, which follows its K tile by KA groups of the ring.
+        // lane x < groups has the page of keys [128 j + x R, + R) of the next tile j
         const int* table = p.c.table + w.b * p.c.table_stride;
-        const int grp = lane % 16;
         auto page_of = [&](int j) -> int {
-          const int key = (w.tile0 + j) * kTileKeys + grp * R;  // lengths stay 1024 below INT_MAX
-          if (grp >= groups || j >= N || key >= w.len) return 0;
+          const int key = (w.tile0 + j) * kTileKeys + lane * R;  // lengths stay 1024 below INT_MAX
+          if (lane >= groups || j >= N || key >= w.len) return 0;
           return min(max(__ldg(table + key / p.c.page_size), 0), p.c.num_pages - 1);
         };
-        const int lead = lane < 16 ? KA : 0;  // K lanes look at tile g + KA, V lanes at tile g
-        int page = page_of(lead - KA < 0 ? N : lead - KA);
+        int page = page_of(0);
         for (int g = -KA; g < N && ok; ++g) {
-          const bool has_v = g >= 0, has_k = g + KA < N;
+          if (KA > 1 && g < 0 && g + KA >= N) continue;  // neither K nor V
           const int j = g + lead;
-          const int page_next = g + 1 + lead >= 0 ? page_of(g + 1 + lead) : 0;
-          if (KA > 1 && !has_v && !has_k) { page = page_next; continue; }
+          const bool mine = j >= 0 && j < N;
           if (!warp_wait_phase(bar(L::kKVEmpty + ring.stage), ring.phase ^ 1u, ctl, kStatusTimeoutLoad)) { ok = false; break; }
           const uint32_t fb = bar(L::kKVFull + ring.stage);
-          auto tile_bytes = [&](int t) -> uint32_t {  // whole groups up to the last key
-            const int left = w.len - (w.tile0 + t) * kTileKeys;
-            return left >= kTileKeys ? kTileBytes : static_cast<uint32_t>((left + R - 1) & -R) * 256u;
-          };
-          if (lane == 0)
-            mbar_arrive_expect_tx(fb, (has_v ? tile_bytes(g) : 0u) + (has_k ? tile_bytes(g + KA) : 0u));
-          st.arm(ring.stage, ring.phase);
-          __syncwarp();
-          const int key = (w.tile0 + j) * kTileKeys + grp * R;
-          if (grp < groups && j >= 0 && j < N && key < w.len) {
-            const uint32_t dst = sbase + L::kKV + ring.stage * L::kSlotBytes + (lane < 16 ? kTileBytes : 0) + grp * R * 128;
-            const CUtensorMap* map = lane < 16 ? &tm_k : &tm_v;
-            const int slot = key % p.c.page_size;
-            tma_load_4d(dst, map, fb, 0, w.h, slot, page, pol_kv);
-            tma_load_4d(dst + kBoxBytes, map, fb, 64, w.h, slot, page, pol_kv);
+          if (mine) {
+            const int left = w.len - (w.tile0 + j) * kTileKeys;  // whole boxes up to the last key
+            if (lane == 0) mbar_arrive_expect_tx(fb, left >= kTileKeys ? kTileBytes : ((left + R - 1) & -R) * 256u);
+            st.arm(ring.stage, ring.phase);
+            __syncwarp();
+            if (lane < groups && lane * R < left) {
+              const uint32_t dst = sbase + L::kKV + ring.stage * L::kSlotBytes + (side_v ? 0 : kTileBytes) + lane * R * 128;
+              const int slot = ((w.tile0 + j) * kTileKeys + lane * R) % p.c.page_size;
+              tma_load_4d(dst, map, fb, 0, w.h, slot, page, pol_kv);
+              tma_load_4d(dst + kBoxBytes, map, fb, 64, w.h, slot, page, pol_kv);
+            }
+            __syncwarp();
+            page = page_of(j + 1);
+            if (side_v && j + 1 == N && left < kTileKeys) {
+              // slots past the end may hold NaN, and 0 * NaN in P V would reach the result
+              if (!warp_wait_phase(fb, ring.phase, ctl, kStatusTimeoutLoad)) { ok = false; break; }
+              uint8_t* v = smem + L::kKV + ring.stage * L::kSlotBytes;
+              for (int x = left * 8 + lane; x < kTileKeys * 8; x += 32) {
+                reinterpret_cast<uint4*>(v)[x] = make_uint4(0u, 0u, 0u, 0u);
+                reinterpret_cast<uint4*>(v + kBoxBytes)[x] = make_uint4(0u, 0u, 0u, 0u);
+              }
+              fence_proxy_async_smem();
+              __syncwarp();
+              if (lane == 0) mbar_arrive(bar(L::kVFix + ring.stage));
+            }
+          } else if (lane == 0) {
+            mbar_arrive(fb);
           }
-          __syncwarp();
-          page = page_next;
           ring.advance<Slots>();
         }
       }
@@ -489,33 +501,6 @@ __global__ void __launch_bounds__(384, 1)
         mbar_wait(bar(L::kTeardown), 0, drain, kStatusTimeoutDrain);
       }
       __syncwarp();
-    } else if (warp == 10) {
-      // ================== zeros for V rows past the end ==================
-      // It follows every group of the ring (and releases each, so that it stays within one round of it).
-      Ring ring;
-      bool ok = true;
-      Piece w;
-      while (ok && next_piece(&w)) {
-        const int N = max(tile_steps(w, 0), QTiles > 1 ? tile_steps(w, 1) : 0);
-        if (N == 0) continue;
-        const int64_t first = static_cast<int64_t>(w.tile0 + N - 1) * kTileKeys;  // of the last V tile
-        const int row = first + kTileKeys > w.len ? static_cast<int>(w.len - first) : kTileKeys;
-        for (int left = N + min(KA, N); left > 0; --left) {
-          if (!warp_wait_phase(bar(L::kKVFull + ring.stage), ring.phase, ctl, kStatusTimeoutLoad)) { ok = false; break; }
-          if (left == 1 && row < kTileKeys) {
-            uint8_t* v = smem + L::kKV + ring.stage * L::kSlotBytes;
-            for (int x = row * 8 + lane; x < kTileKeys * 8; x += 32) {
-              reinterpret_cast<uint4*>(v)[x] = make_uint4(0u, 0u, 0u, 0u);
-              reinterpret_cast<uint4*>(v + kBoxBytes)[x] = make_uint4(0u, 0u, 0u, 0u);
-            }
-            fence_proxy_async_smem();
-            __syncwarp();
-            if (lane == 0) mbar_arrive(bar(L::kVFix + ring.stage));
-          }
-          if (lane == 0) mbar_arrive(bar(L::kKVEmpty + ring.stage));
-          ring.advance<Slots>();
-        }
-      }
     } else {
       // ============================== schedule ==============================
       int4 cut = make_int4(0, 0, 0, -1);
