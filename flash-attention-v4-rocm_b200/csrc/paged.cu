@@ -55,8 +55,10 @@ int sm_count(int* sms) {
     int n = 0;
     e = cudaDeviceGetAttribute(&n, cudaDevAttrMultiProcessorCount, dev);
     if (e != cudaSuccess) return e;
-    e = cudaFuncSetAttribute(paged_attn_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, kPagedSmem);
-    if (e != cudaSuccess) return e;
+    for (auto kernel : {paged_attn_kernel<false>, paged_attn_kernel<true>}) {
+      e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, kPagedSmem);
+      if (e != cudaSuccess) return e;
+    }
     e = cudaFuncSetAttribute(paged_tile_kernel<1>, cudaFuncAttributeMaxDynamicSharedMemorySize, PagedTileLayout<1>::kAlloc);
     if (e != cudaSuccess) return e;
     e = cudaFuncSetAttribute(paged_tile_kernel<2>, cudaFuncAttributeMaxDynamicSharedMemorySize, PagedTileLayout<2>::kAlloc);
@@ -131,10 +133,13 @@ int q_tiles(long long tokens, int group) {
 }
 
 // Workspace: counters first (their place never changes, so that any call may follow any other), then the
-// pieces of cut units (of whichever kernel needs more), then the first of a prefixed call's two results.
+// pieces of units that paged_attn_kernel cuts (a prefixed call's two launches overlap, and have their own),
+// those of paged_tile_kernel, then the first of a prefixed call's two results.
 struct PagedSpace {
-  size_t part_o, part_ml, tile_o, tile_ml, cut, first_o, first_lse, total;
+  size_t part, tile_o, tile_ml, cut, first_o, first_lse, total;
   static constexpr size_t kCounters = 4096;
+  static constexpr size_t kPartO = size_t(2) * kMaxGrid * kPagedRows * 128 * sizeof(float);
+  static constexpr size_t kPart = kPartO + size_t(2) * kMaxGrid * kPagedRows * 2 * sizeof(float);
 };
 static_assert(2 * kMaxGrid * sizeof(uint32_t) <= PagedSpace::kCounters, "two calls' counters");
 static_assert(kMaxSms <= 256, "paged_join_kernel reads one cut unit per thread");
@@ -143,9 +148,8 @@ PagedSpace paged_space(const Fav4PagedArgs& a) {
   int tiles = q_tiles(a.max_sq, group);
   if (a.prefix_pages && q_tiles(a.total_q, group) > tiles) tiles = q_tiles(a.total_q, group);
   PagedSpace s;
-  s.part_o = PagedSpace::kCounters;
-  s.part_ml = s.part_o + size_t(2) * kMaxGrid * kPagedRows * 128 * sizeof(float);
-  s.tile_o = s.part_ml + size_t(2) * kMaxGrid * kPagedRows * 2 * sizeof(float);
+  s.part = PagedSpace::kCounters;
+  s.tile_o = s.part + (a.prefix_pages ? 2 : 1) * PagedSpace::kPart;
   s.tile_ml = s.tile_o + size_t(2) * kMaxSms * tiles * kBlockM * 128 * sizeof(float);
   s.cut = s.tile_ml + size_t(2) * kMaxSms * tiles * kBlockM * 2 * sizeof(float);
   s.first_o = s.cut + round256(kMaxSms * sizeof(int4));
@@ -199,7 +203,7 @@ int launch_rows(const PagedParams& p, const PagedSpace& sp, uint8_t* ws, int sms
   const int tiles = mapped ? q_tiles(p.max_sq, p.group) : 0;
   if (tiles == 1) return launch_tiles<1>(p, sp, ws, sms, stream);
   if (tiles == 2) return launch_tiles<2>(p, sp, ws, sms, stream);
-  return launch(paged_attn_kernel, sms * kPagedPerSm, kPagedWarps * 32, kPagedSmem, stream, p);
+  return launch(p.add_o ? paged_attn_kernel<true> : paged_attn_kernel<false>, sms * kPagedPerSm, kPagedWarps * 32, kPagedSmem, stream, p);
 }
 
 int launch_paged(const Fav4PagedArgs& a, int causal, uint8_t* ws, cudaStream_t stream) {
@@ -212,8 +216,8 @@ int launch_paged(const Fav4PagedArgs& a, int causal, uint8_t* ws, cudaStream_t s
   p.q = static_cast<const __nv_bfloat16*>(a.q);
   p.q_ts = a.q_token_stride;
   p.q_hs = a.q_head_stride;
-  p.part_o = reinterpret_cast<float*>(ws + sp.part_o);
-  p.part_ml = reinterpret_cast<float*>(ws + sp.part_ml);
+  p.part_o = reinterpret_cast<float*>(ws + sp.part);
+  p.part_ml = reinterpret_cast<float*>(ws + sp.part + PagedSpace::kPartO);
   p.arrived = reinterpret_cast<uint32_t*>(ws);
   p.heads = a.heads;
   p.group = a.heads / a.cache.kv_heads;
@@ -238,6 +242,8 @@ int launch_paged(const Fav4PagedArgs& a, int causal, uint8_t* ws, cudaStream_t s
   first.o = nullptr;
   first.o32 = reinterpret_cast<float*>(ws + sp.first_o);
   first.lse = reinterpret_cast<float*>(ws + sp.first_lse);
+  first.part_o = reinterpret_cast<float*>(ws + sp.part + PagedSpace::kPart);
+  first.part_ml = reinterpret_cast<float*>(ws + sp.part + PagedSpace::kPart + PagedSpace::kPartO);
   first.arrived += kMaxGrid;
   rc = launch_rows(first, sp, ws, sms, stream);
   if (rc) return rc;

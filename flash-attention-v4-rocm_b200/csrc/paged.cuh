@@ -15,9 +15,13 @@ namespace fav4 {
 // Every kernel here is launched as a programmatic dependent of whatever precedes it on its stream: it may be
 // scheduled while that still runs, waits here before it reads or writes any memory that others use, and
 // lets its own successor be scheduled at once.
-__device__ __forceinline__ void wait_for_predecessor() {
-  asm volatile("griddepcontrol.wait;" ::: "memory");
+__device__ __forceinline__ void grid_wait() { asm volatile("griddepcontrol.wait;" ::: "memory"); }
+__device__ __forceinline__ void grid_launch_dependents() {
   asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
+}
+__device__ __forceinline__ void wait_for_predecessor() {
+  grid_wait();
+  grid_launch_dependents();
 }
 
 struct PagedCacheView {
@@ -44,17 +48,24 @@ __host__ __device__ __forceinline__ int64_t quotient(int64_t a, int64_t b) {
   return divide64(a, b);
 }
 
+// A load through L1 (the ordinary case) or past it.
+template <bool PastL1, typename T>
+__device__ __forceinline__ T load(const T* p) {
+  return PastL1 ? __ldcg(p) : __ldg(p);
+}
+
+template <bool PastL1 = false>
 __device__ __forceinline__ SeqView seq_view(const PagedCacheView& c, const int* cu, int total_q, int max_sq, int b) {
   SeqView s;
   if (cu != nullptr) {
-    s.q0 = min(max(__ldg(cu + b), 0), total_q);
-    s.sq = min(min(max(__ldg(cu + b + 1), s.q0), total_q) - s.q0, max_sq);
+    s.q0 = min(max(load<PastL1>(cu + b), 0), total_q);
+    s.sq = min(min(max(load<PastL1>(cu + b + 1), s.q0), total_q) - s.q0, max_sq);
   } else {  // one sequence of all rows
     s.q0 = 0;
     s.sq = total_q;
   }
   const int64_t cap = static_cast<int64_t>(c.max_pages) * c.page_size;
-  s.len = static_cast<int>(min(static_cast<int64_t>(max(__ldg(c.lens + b), 0)), cap));
+  s.len = static_cast<int>(min(static_cast<int64_t>(max(load<PastL1>(c.lens + b), 0)), cap));
   return s;
 }
 
@@ -327,11 +338,11 @@ __device__ __noinline__ void finish_row(const PagedParams& p, const RowPlace& at
   const int64_t row = static_cast<int64_t>(at.token) * p.heads + at.head;
   const int64_t lse_at = static_cast<int64_t>(at.head) * p.total_q + at.token;
   if (p.add_o != nullptr) {
-    const float other = p.add_lse[lse_at] * 1.4426950408889634f;  // base 2; -inf where that result saw no key
+    const float other = __ldcg(p.add_lse + lse_at) * 1.4426950408889634f;  // base 2; -inf where that result saw no key
     const float top = fmaxf(m, other);
     if (top != -INFINITY) {
       const float w = exp2f(m - top), x = exp2f(other - top);
-      const float4 b = *reinterpret_cast<const float4*>(p.add_o + row * 128 + lane * 4);
+      const float4 b = __ldcg(reinterpret_cast<const float4*>(p.add_o + row * 128 + lane * 4));
       // where x is 0 the other row is zero
       acc = make_float4(acc.x * w + b.x * x, acc.y * w + b.y * x, acc.z * w + b.z * x, acc.w * w + b.w * x);
       l = l * w + x;
@@ -382,6 +393,13 @@ __device__ __forceinline__ T block_scan(T v, T* tmp, T* sum) {
 // Byte offset of 4-column piece c of row r of a 16 x 128 FP32 tile in a ring slot, spread over the banks.
 __device__ __forceinline__ int tile_at(int r, int c) { return r * 512 + ((c ^ (r & 7)) * 16); }
 
+// Joined: the result is joined with another one (add_o), which the predecessor computes from the same inputs.
+// That kernel let this one be scheduled only after its own wait, so everything but its result (and the
+// outputs, whose last reader may have been before it) is there already and only the rows' ends wait: the
+// launch, the first copies and the products overlap with it (64 sequences behind 32768 keys: 64 -> 54 us).
+// The inputs are then read through L2, past lines that an SM may hold from before; that costs a short launch
+// 1 us, so the ordinary kernel keeps L1.
+template <bool Joined>
 __global__ void __launch_bounds__(kPagedWarps * 32, 2) paged_attn_kernel(const __grid_constant__ PagedParams p) {
   extern __shared__ __align__(1024) uint8_t smem[];
   __shared__ __align__(16) PagedPiece list[kPagedList];
@@ -395,7 +413,8 @@ __global__ void __launch_bounds__(kPagedWarps * 32, 2) paged_attn_kernel(const _
   const int mi = lane / 8, mr = lane % 8;    // ldmatrix: matrix and row that this lane addresses
   const int cl = lane % 16, rl = lane / 16;  // copies: 16-byte piece cl of rows rl + 2 j
   const uint32_t ring = smem_addr(smem) + warp * kPagedRing;
-  wait_for_predecessor();
+  if (Joined) grid_launch_dependents();
+  else wait_for_predecessor();
 
   int64_t total = 0, per = 0, begin = 0, end = 0;
   for (int round = 0;; ++round) {
@@ -407,7 +426,7 @@ __global__ void __launch_bounds__(kPagedWarps * 32, 2) paged_attn_kernel(const _
       for (int b0 = 0; b0 < p.c.batch; b0 += kPagedWarps * 32) {
         const int b = b0 + tid;
         SeqView s = {0, 0, 0};
-        if (b < p.c.batch) s = seq_view(p.c, p.cu, p.total_q, p.max_sq, b);
+        if (b < p.c.batch) s = seq_view<Joined>(p.c, p.cu, p.total_q, p.max_sq, b);
         const int64_t work = paged_seq_work(p, s);
         int64_t sum;
         const int64_t first_tile = base + block_scan(work, scan64, &sum) - work;  // of this sequence
@@ -466,7 +485,7 @@ __global__ void __launch_bounds__(kPagedWarps * 32, 2) paged_attn_kernel(const _
       }
     }
     const int count = min(pieces - round * kPagedList, kPagedList);
-    if (count <= 0) return;
+    if (count <= 0) break;
     __syncthreads();
 
     // ---- copies: this warp's 16-key groups of all listed pieces, kPagedStages - 1 ahead of their use ----
@@ -476,7 +495,7 @@ __global__ void __launch_bounds__(kPagedWarps * 32, 2) paged_attn_kernel(const _
     auto pages_from = [&](int i, int s0) -> int {
       if (i >= count || s0 + lane >= steps_of(i)) return 0;
       const int key = list[i].key_begin + (warp + kPagedWarps * (s0 + lane)) * 16;
-      const int page = __ldg(p.c.table + list[i].b * p.c.table_stride + key / p.c.page_size);
+      const int page = load<Joined>(p.c.table + list[i].b * p.c.table_stride + key / p.c.page_size);
       return min(max(page, 0), p.c.num_pages - 1);
     };
     auto skip_empty = [&](int i) {
@@ -540,8 +559,8 @@ __global__ void __launch_bounds__(kPagedWarps * 32, 2) paged_attn_kernel(const _
             p.q + (w.q0 + token) * p.q_ts + (w.h * p.group + r - token * p.group) * p.q_hs + t4 * 2;
 #pragma unroll
         for (int k = 0; k < 8; ++k) {
-          qf[k][u] = live ? __ldg(reinterpret_cast<const uint32_t*>(src + k * 16)) : 0u;
-          qf[k][u + 2] = live ? __ldg(reinterpret_cast<const uint32_t*>(src + k * 16 + 8)) : 0u;
+          qf[k][u] = live ? load<Joined>(reinterpret_cast<const uint32_t*>(src + k * 16)) : 0u;
+          qf[k][u + 2] = live ? load<Joined>(reinterpret_cast<const uint32_t*>(src + k * 16 + 8)) : 0u;
         }
       }
     };
@@ -650,6 +669,7 @@ __global__ void __launch_bounds__(kPagedWarps * 32, 2) paged_attn_kernel(const _
       }
       if (lane == 0) free_slot[warp] = spare;
       __syncthreads();
+      if (Joined) grid_wait();  // the other result is complete
       const PagedPiece& w = list[i];
       const int rows = static_cast<int>(min(static_cast<int64_t>(kPagedRows), static_cast<int64_t>(sq) * p.group - r0));
       const bool whole = w.cnt == w.n;
@@ -757,9 +777,10 @@ __global__ void __launch_bounds__(kPagedWarps * 32, 2) paged_attn_kernel(const _
       __syncthreads();  // the slots that hold the O tiles are the next to be copied to
     }
     cp_async_wait<0>();
-    if (pieces - round * kPagedList <= kPagedList) return;
+    if (pieces - round * kPagedList <= kPagedList) break;
     __syncthreads();  // the list is written anew
   }
+  if (Joined) grid_wait();  // no block ends before its predecessor has: the successor waits for this grid only
 }
 
 }  // namespace fav4
