@@ -8,6 +8,7 @@
 #pragma once
 #include <cuda_bf16.h>
 #include <cstdint>
+#include "paged_schedule.h"
 #include "sm100.cuh"
 
 namespace fav4 {
@@ -33,39 +34,30 @@ struct PagedCacheView {
   int num_pages, page_size, max_pages, kv_heads, batch;
 };
 
-// Rows, keys and offsets of one sequence, clamped so that malformed offsets, lengths or page numbers
-// can give wrong rows but no access outside the tensors.
-struct SeqView {
-  int q0, sq, len;
-};
-
-// a / b for a >= 0, b > 0. Work counts are 64-bit, but nearly always small: a 64-bit division costs several
-// times a 32-bit one, and the schedules wait for theirs. The long way is kept out of line: code that a kernel
-// fetches once, at its start, costs it more than the arithmetic.
-__host__ __device__ __noinline__ inline int64_t divide64(int64_t a, int64_t b) { return a / b; }
-__host__ __device__ __forceinline__ int64_t quotient(int64_t a, int64_t b) {
-  if (((a | b) >> 32) == 0) return static_cast<uint32_t>(a) / static_cast<uint32_t>(b);
-  return divide64(a, b);
-}
-
 // A load through L1 (the ordinary case) or past it.
 template <bool PastL1, typename T>
 __device__ __forceinline__ T load(const T* p) {
   return PastL1 ? __ldcg(p) : __ldg(p);
 }
 
+// Offsets, lengths and rows of sequence b, clamped so that malformed ones can give wrong rows but no access
+// outside the tensors. Rows past max_sq are not computed; with a mask, nor are the keys that only they see
+// (the last row's key stays the last one, so the others keep their places; the length may become negative).
 template <bool PastL1 = false>
-__device__ __forceinline__ SeqView seq_view(const PagedCacheView& c, const int* cu, int total_q, int max_sq, int b) {
+__device__ __forceinline__ SeqView seq_view(const PagedCacheView& c, const int* cu, int total_q, int max_sq,
+                                            int causal, int b) {
   SeqView s;
+  const int64_t cap = static_cast<int64_t>(c.max_pages) * c.page_size;
+  s.len = static_cast<int>(min(static_cast<int64_t>(max(load<PastL1>(c.lens + b), 0)), cap));
   if (cu != nullptr) {
     s.q0 = min(max(load<PastL1>(cu + b), 0), total_q);
-    s.sq = min(min(max(load<PastL1>(cu + b + 1), s.q0), total_q) - s.q0, max_sq);
+    const int rows = min(max(load<PastL1>(cu + b + 1), s.q0), total_q) - s.q0;
+    s.sq = min(rows, max_sq);
+    if (causal) s.len -= rows - s.sq;
   } else {  // one sequence of all rows
     s.q0 = 0;
     s.sq = total_q;
   }
-  const int64_t cap = static_cast<int64_t>(c.max_pages) * c.page_size;
-  s.len = static_cast<int>(min(static_cast<int64_t>(max(load<PastL1>(c.lens + b), 0)), cap));
   return s;
 }
 
@@ -426,7 +418,7 @@ __global__ void __launch_bounds__(kPagedWarps * 32, 2) paged_attn_kernel(const _
       for (int b0 = 0; b0 < p.c.batch; b0 += kPagedWarps * 32) {
         const int b = b0 + tid;
         SeqView s = {0, 0, 0};
-        if (b < p.c.batch) s = seq_view<Joined>(p.c, p.cu, p.total_q, p.max_sq, b);
+        if (b < p.c.batch) s = seq_view<Joined>(p.c, p.cu, p.total_q, p.max_sq, p.causal, b);
         const int64_t work = paged_seq_work(p, s);
         int64_t sum;
         const int64_t first_tile = base + block_scan(work, scan64, &sum) - work;  // of this sequence

@@ -1,0 +1,84 @@
+// The arithmetic of the paged attention's schedules, for the kernels and for a host compiler.
+#pragma once
+#include <cstdint>
+
+#ifdef __CUDACC__
+#define FAV4_HD __host__ __device__ __forceinline__
+#define FAV4_HD_CALL __host__ __device__ __noinline__ inline
+#else
+#define FAV4_HD inline
+#define FAV4_HD_CALL inline
+#endif
+
+namespace fav4 {
+
+// One sequence: its first row of Q, its rows, its keys.
+struct SeqView {
+  int q0, sq, len;
+};
+
+// a / b for a >= 0, b > 0. Work counts are 64-bit, but nearly always small: a 64-bit division costs several
+// times a 32-bit one, and the schedules wait for theirs. The long way is kept out of line: code that a kernel
+// fetches once, at its start, costs it more than the arithmetic.
+FAV4_HD_CALL int64_t divide64(int64_t a, int64_t b) { return a / b; }
+FAV4_HD int64_t quotient(int64_t a, int64_t b) {
+  if (((a | b) >> 32) == 0) return static_cast<uint32_t>(a) / static_cast<uint32_t>(b);
+  return divide64(a, b);
+}
+
+// paged_tile_kernel: a unit is `bt` tokens of a sequence (the last one: what is left) and takes a step for
+// each 128-key tile up to its last visible key; one that sees no key keeps a step, which writes its zero rows.
+constexpr int kTileKeys = 128;
+
+// sum over j < n of floor((a j + c) / 128), for a, c >= 0, by the steps of Euclid's algorithm. Blocks wait
+// for it, so the first step (by 128) has no division and the others one each: their c and a are below 128.
+FAV4_HD_CALL int64_t floor_sum128(int64_t n, int64_t a, int64_t c) {
+  if (n <= 0) return 0;
+  int64_t s = n * (n - 1) / 2 * (a >> 7) + n * (c >> 7);
+  int m = 128, r = static_cast<int>(a & 127), d = static_cast<int>(c & 127);
+  while (true) {
+    const int64_t y = r * n + d;
+    if (y < m) break;
+    const int64_t k = m == 128 ? y >> 7 : quotient(y, m);
+    d = static_cast<int>(y - k * m);
+    n = k;
+    const int q = static_cast<int>(static_cast<unsigned>(m) / static_cast<unsigned>(r));  // r > 0: y >= m > d
+    const int e = static_cast<int>(static_cast<unsigned>(d) / static_cast<unsigned>(r));
+    s += n * (n - 1) / 2 * q + n * e;
+    const int t = m - q * r;
+    d -= e * r;
+    m = r;
+    r = t;
+  }
+  return s;
+}
+
+FAV4_HD int steps_up_to(int64_t keys) {
+  return keys <= 0 ? 1 : static_cast<int>((keys + kTileKeys - 1) / kTileKeys);
+}
+// Steps of unit r of a sequence, and of units 0 .. r - 1.
+FAV4_HD int unit_steps(const SeqView& s, int causal, int bt, int r) {
+  const int64_t full = (static_cast<int64_t>(r) + 1) * bt;
+  const int64_t last = full < s.sq ? full : s.sq;
+  return steps_up_to(causal ? static_cast<int64_t>(s.len) - s.sq + last : s.len);
+}
+FAV4_HD_CALL int64_t units_steps(const SeqView& s, int causal, int bt, int64_t r) {
+  if (r <= 0) return 0;
+  if (!causal) return r * steps_up_to(s.len);
+  const int64_t units = quotient(static_cast<int64_t>(s.sq) + bt - 1, bt);
+  int64_t sum = 0;
+  if (r == units) {  // the last one ends with the sequence, the others after a whole number of bt tokens
+    sum = steps_up_to(s.len);
+    --r;
+  }
+  const int64_t past = static_cast<int64_t>(s.len) - s.sq;
+  int64_t ones = past <= kTileKeys ? quotient(kTileKeys - past, bt) : 0;  // units that end within the first tile
+  if (ones > r) ones = r;
+  // units ones .. r - 1: ceil((past + (j + 1) bt) / 128)
+  return sum + ones + floor_sum128(r - ones, bt, past + (ones + 1) * bt + kTileKeys - 1);
+}
+FAV4_HD int64_t tile_seq_work(const SeqView& s, int causal, int bt) {
+  return s.sq == 0 ? 0 : units_steps(s, causal, bt, quotient(static_cast<int64_t>(s.sq) + bt - 1, bt));
+}
+
+}  // namespace fav4

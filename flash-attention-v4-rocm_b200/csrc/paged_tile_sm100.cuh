@@ -28,7 +28,6 @@
 
 namespace fav4 {
 
-constexpr int kTileKeys = 128;
 constexpr int kPieceSlots = 4;
 constexpr uint32_t kTileSoftmaxRegs = 208;  // 128 * (2 * 208 + 88) = 384 * 168
 constexpr uint32_t kTileOtherRegs = 88;
@@ -64,57 +63,6 @@ struct Piece {
   int pad[7];
 };
 static_assert(sizeof(Piece) == 64, "four 16-byte words");
-
-// sum over j < n of floor((a j + c) / 128), for a, c >= 0, by the steps of Euclid's algorithm. Blocks wait
-// for it, so the first step (by 128) has no division and the others one each: their c and a are below 128.
-__host__ __device__ __noinline__ inline int64_t floor_sum128(int64_t n, int64_t a, int64_t c) {
-  if (n <= 0) return 0;
-  int64_t s = n * (n - 1) / 2 * (a >> 7) + n * (c >> 7);
-  int m = 128, r = static_cast<int>(a & 127), d = static_cast<int>(c & 127);
-  while (true) {
-    const int64_t y = r * n + d;
-    if (y < m) break;
-    const int64_t k = m == 128 ? y >> 7 : quotient(y, m);
-    d = static_cast<int>(y - k * m);
-    n = k;
-    const int q = static_cast<int>(static_cast<unsigned>(m) / static_cast<unsigned>(r));  // r > 0: y >= m > d
-    const int e = static_cast<int>(static_cast<unsigned>(d) / static_cast<unsigned>(r));
-    s += n * (n - 1) / 2 * q + n * e;
-    const int t = m - q * r;
-    d -= e * r;
-    m = r;
-    r = t;
-  }
-  return s;
-}
-
-__host__ __device__ __forceinline__ int steps_up_to(int64_t keys) {
-  return keys <= 0 ? 1 : static_cast<int>((keys + kTileKeys - 1) / kTileKeys);
-}
-// Steps of unit r of a sequence, and of units 0 .. r - 1.
-__host__ __device__ __forceinline__ int unit_steps(const SeqView& s, int causal, int bt, int r) {
-  const int64_t full = (static_cast<int64_t>(r) + 1) * bt;
-  const int64_t last = full < s.sq ? full : s.sq;
-  return steps_up_to(causal ? static_cast<int64_t>(s.len) - s.sq + last : s.len);
-}
-__host__ __device__ __noinline__ inline int64_t units_steps(const SeqView& s, int causal, int bt, int64_t r) {
-  if (r <= 0) return 0;
-  if (!causal) return r * steps_up_to(s.len);
-  const int64_t units = quotient(static_cast<int64_t>(s.sq) + bt - 1, bt);
-  int64_t sum = 0;
-  if (r == units) {  // the last one ends with the sequence, the others after a whole number of bt tokens
-    sum = steps_up_to(s.len);
-    --r;
-  }
-  const int64_t past = static_cast<int64_t>(s.len) - s.sq;
-  int64_t ones = past <= kTileKeys ? quotient(kTileKeys - past, bt) : 0;  // units that end within the first tile
-  if (ones > r) ones = r;
-  // units ones .. r - 1: ceil((past + (j + 1) bt) / 128)
-  return sum + ones + floor_sum128(r - ones, bt, past + (ones + 1) * bt + kTileKeys - 1);
-}
-__host__ __device__ __forceinline__ int64_t tile_seq_work(const SeqView& s, int causal, int bt) {
-  return s.sq == 0 ? 0 : units_steps(s, causal, bt, quotient(static_cast<int64_t>(s.sq) + bt - 1, bt));
-}
 
 template <int QTiles>
 struct PagedTileLayout {
@@ -152,7 +100,11 @@ __global__ void __launch_bounds__(384, 1)
   extern __shared__ __align__(1024) uint8_t smem[];
   const uint32_t sbase = smem_addr(smem);
   if (sbase & 1023) {  // the swizzled tiles need it; there is no room to round up
-    if (threadIdx.x == 0) atomicOr(tp.status, kStatusSmemAlign);
+    wait_for_predecessor();
+    if (threadIdx.x == 0) {
+      atomicOr(tp.status, kStatusSmemAlign);
+      tp.cut[blockIdx.x] = make_int4(0, 0, 0, -1);
+    }
     return;
   }
   const uint32_t bar0 = sbase + L::kBar;
@@ -207,7 +159,7 @@ __global__ void __launch_bounds__(384, 1)
     for (int b0 = 0; b0 < p.c.batch; b0 += 384) {
       const int b = b0 + threadIdx.x;
       SeqView view = {0, 0, 0};
-      if (b < p.c.batch) view = seq_view(p.c, p.cu, p.total_q, p.max_sq, b);
+      if (b < p.c.batch) view = seq_view(p.c, p.cu, p.total_q, p.max_sq, p.causal, b);
       const int64_t head_work = tile_seq_work(view, p.causal, bt), mine = head_work * p.c.kv_heads;
       int64_t v = mine;
 #pragma unroll
@@ -573,7 +525,7 @@ __global__ void __launch_bounds__(384, 1)
           if (pos >= end) break;
           base += head_work * p.c.kv_heads;
           ++b;
-          s = seq_view(p.c, p.cu, p.total_q, p.max_sq, b);
+          s = seq_view(p.c, p.cu, p.total_q, p.max_sq, p.causal, b);
           head_work = tile_seq_work(s, p.causal, bt);
         }
       }

@@ -446,3 +446,38 @@ def test_many_short_sequences(cuda):
     x = Batch([1] * b, keys, 8, 8, 16, seed=54)
     o, lse = attend(x)
     check_attention(o, lse, x.reference())
+
+
+@pytest.mark.parametrize("sq,keys,bound", [([3, 1, 6], [300, 40, 5], 2), ([90, 20, 300], [500, 20, 310], 40)])
+@pytest.mark.parametrize("causal", [True, False])
+def test_rows_past_the_bound_are_left_alone(cuda, sq, keys, bound, causal):
+    # max_sq below a sequence's rows: the first rows are right, the others are not written
+    x = Batch(sq, keys, 8, 2, 16, seed=55)
+    out = torch.full_like(x.q, 7.0)
+    o, lse = paged.attention(x.q, x.k_cache, x.v_cache, x.table, x.lens, x.cu, bound, causal=causal, out=out,
+                             return_lse=True)
+    want_o, want_lse, w = x.reference(causal)
+    rows = torch.cat([torch.arange(int(a), int(a) + min(n, bound)) for a, n in zip(x.cu.cpu(), sq)])
+    check_attention(o[rows], lse[:, rows], (want_o[rows], want_lse[:, rows], w[rows]))
+    left = torch.ones(sum(sq), dtype=torch.bool)
+    left[rows] = False
+    assert (o[left] == 7.0).all()
+
+
+@pytest.mark.parametrize("sq", [1, 5, 40])
+def test_offsets_past_32_bits(cuda, sq):
+    # pages whose elements lie beyond 2^31 (and bytes beyond 2^32) of a cache
+    h, hk, page, n = 8, 2, 64, 300
+    pages = 2 ** 31 // (page * hk * D) + 40
+    k_cache, v_cache = (torch.empty(pages, page, hk, D, dtype=torch.bfloat16, device=cuda) for _ in range(2))
+    small = Batch([sq], [n], h, hk, page, seed=56)
+    last = small.k_cache.shape[0]
+    k_cache[-last:], v_cache[-last:] = small.k_cache, small.v_cache
+    table = (small.table + (pages - last)).to(torch.int32)
+    o, lse = paged.attention(small.q, k_cache, v_cache, table, small.lens, small.cu, sq, return_lse=True)
+    check_attention(o, lse, small.reference())
+    k = torch.randn(sq, hk, D, device=cuda).bfloat16()
+    paged.append(small.q, k, -k, k_cache, v_cache, table, small.lens, small.cu)
+    at = torch.arange(n - sq, n, device=cuda)
+    rows = table[0].long()[at // page]
+    assert torch.equal(k_cache[rows, at % page], k) and torch.equal(v_cache[rows, at % page], -k)

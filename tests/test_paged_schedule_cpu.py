@@ -1,0 +1,53 @@
+"""CPU test of the arithmetic behind the paged attention's schedule (csrc/paged_schedule.h): the closed forms that
+the blocks locate their work with, against sums over every unit."""
+import subprocess
+from pathlib import Path
+
+import fav4_bshd as F
+
+PROGRAM = r"""
+#include <cstdio>
+#include <cstdlib>
+#include "paged_schedule.h"
+using namespace fav4;
+int main() {
+  srand(1);
+  const int groups[] = {1, 2, 3, 4, 5, 6, 7, 8, 12, 16, 32, 100, 128};
+  long checked = 0;
+  for (int it = 0; it < 20000; ++it) {
+    SeqView s;
+    s.q0 = 0;
+    s.sq = 1 + rand() % (it % 3 ? 300 : 5000);
+    s.len = it % 5 == 0 ? rand() % (s.sq + 1) : it % 7 == 0 ? s.sq : s.sq + rand() % 6000;
+    if (it % 11 == 0) s.len = -rand() % 500;  // all rows before the first key
+    const int bt = 128 / groups[rand() % 13] * (1 + rand() % 2), causal = it % 4 != 0;
+    const int units = (s.sq + bt - 1) / bt;
+    long sum = 0;
+    for (int r = 0; r <= units; ++r, ++checked) {
+      if (units_steps(s, causal, bt, r) != sum) {
+        printf("sq %d len %d bt %d causal %d: %ld steps before unit %d, not %ld\n", s.sq, s.len, bt, causal, sum, r,
+               (long)units_steps(s, causal, bt, r));
+        return 1;
+      }
+      if (r == units) break;
+      const long end = (r + 1L) * bt < s.sq ? (r + 1L) * bt : s.sq, keys = causal ? (long)s.len - s.sq + end : s.len;
+      const long want = keys <= 0 ? 1 : (keys + 127) / 128;
+      if (unit_steps(s, causal, bt, r) != want) return 2;
+      sum += want;
+    }
+    if (tile_seq_work(s, causal, bt) != sum) return 3;
+  }
+  if (quotient(1L << 40, 3) != (1L << 40) / 3 || quotient(7, 1L << 33) != 0 || quotient(4294967295L, 2) != 2147483647L) return 4;
+  printf("%ld\n", checked);
+  return 0;
+}
+"""
+
+
+def test_closed_forms(tmp_path):
+    src, exe = tmp_path / "schedule.cpp", tmp_path / "schedule"
+    src.write_text(PROGRAM)
+    subprocess.run(["g++", "-O1", "-std=c++17", f"-I{F.PKG_ROOT / 'csrc'}", str(src), "-o", str(exe)], check=True)
+    r = subprocess.run([str(exe)], capture_output=True, text=True)
+    assert r.returncode == 0, r.stdout
+    assert int(r.stdout) > 100000
