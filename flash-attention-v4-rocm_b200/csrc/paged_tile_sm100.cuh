@@ -74,7 +74,8 @@ struct PagedTileLayout {
   static constexpr int kQFull = 0, kQEmpty = 1, kKVFull = 2, kKVEmpty = kKVFull + kSlots, kVFix = kKVEmpty + kSlots;
   static constexpr int kSFull = kVFix + kSlots, kPFull = kSFull + 2, kOFull = kPFull + 2, kOEmpty = kOFull + 2;
   static constexpr int kPieceFull = kOEmpty + 2, kPieceEmpty = kPieceFull + kPieceSlots;
-  static constexpr int kTeardown = kPieceEmpty + kPieceSlots;
+  static constexpr int kXFull = kPieceEmpty + kPieceSlots, kXEmpty = kXFull + 1;  // one Q tile: the streams' (m, l)
+  static constexpr int kTeardown = kXEmpty + 1;
   static constexpr int kNumBars = kTeardown + 1;
   static constexpr int kPieces = (kBar + kNumBars * 8 + 15) & ~15;
   static constexpr int kMisc = kPieces + kPieceSlots * 64;  // TMEM base, abort flag, schedule scan
@@ -137,6 +138,8 @@ __global__ void __launch_bounds__(384, 1)
       mbar_init(bar(L::kPieceFull + s), 1);
       mbar_init(bar(L::kPieceEmpty + s), 3 + 8);  // load, MMA and V warps, softmax warps
     }
+    mbar_init(bar(L::kXFull), 8);
+    mbar_init(bar(L::kXEmpty), 8);
     mbar_init(bar(L::kTeardown), 1);
     fence_mbar_init();
   }
@@ -552,7 +555,7 @@ __global__ void __launch_bounds__(384, 1)
     const uint32_t t_o = tmem + lane_off + 256 + i * 128;
     const int col0 = QTiles == 1 ? i * kCols : 0;
     float2* ml_shared = reinterpret_cast<float2*>(smem + L::kMl);  // [stream][row]
-    uint32_t s_par = 0, o_full_par = 0;  // o_full: bit x for O_x
+    uint32_t s_par = 0, o_full_par = 0, x_par = 0;  // o_full: bit x for O_x
     const float scale_log2 = p.scale_log2;
     const int row_token = row / p.group;  // token of this row within the Q tile
     const int row_head = row - row_token * p.group;
@@ -630,11 +633,17 @@ __global__ void __launch_bounds__(384, 1)
       // ------------------------------ epilogue ------------------------------
       float ov[kCols];
       if constexpr (QTiles == 1) {
-        // both streams' (m, l), and whether every warp got here
+        // both streams' (m, l), exchanged with bounded waits like every other: a hardware barrier would wait for
+        // good for a warp that gave up
+        if (!ok || !warp_wait(bar(L::kXEmpty), x_par ^ 1u, ctl, kStatusTimeoutSoftmax)) { ok = false; break; }
         ml_shared[i * 128 + row] = make_float2(m, l);
-        if (!pair_all(1, 256, ok)) { ok = false; break; }
+        __syncwarp();
+        if (lane == 0) mbar_arrive(bar(L::kXFull));
+        if (!warp_wait(bar(L::kXFull), x_par, ctl, kStatusTimeoutSoftmax)) { ok = false; break; }
         const float2 x0 = ml_shared[row], x1 = ml_shared[128 + row];
-        named_sync(1, 256);  // both are read: the next piece may write
+        __syncwarp();
+        if (lane == 0) mbar_arrive(bar(L::kXEmpty));
+        x_par ^= 1u;
         const float top = fmaxf(x0.x, x1.x), zero = top == -INFINITY ? 0.f : top;
         const float a0 = exp2f(x0.x - zero), a1 = exp2f(x1.x - zero);
         m = top;
