@@ -81,4 +81,19 @@ FAV4_HD int64_t tile_seq_work(const SeqView& s, int causal, int bt) {
   return s.sq == 0 ? 0 : units_steps(s, causal, bt, quotient(static_cast<int64_t>(s.sq) + bt - 1, bt));
 }
 
+// A piece costs about as much beside its steps as two of them, so a block that takes only that little of a
+// unit leaves it to its neighbour, unless its whole stretch of `per` steps is short (a quarter at most) or so
+// long that the imbalance would cost more than the piece.
+FAV4_HD int piece_slack(int64_t per) { return per > 32 ? 0 : static_cast<int>(per / 4 < 2 ? per / 4 : 2); }
+// Where a boundary between two blocks, `at` steps into a unit of n, really cuts: at its begin or end if that is
+// at most `slack` steps away. Both blocks ask, so what one leaves the other takes.
+FAV4_HD int snap(int64_t at, int n, int slack) {
+  if (at <= slack) return 0;
+  return at >= n - slack ? n : static_cast<int>(at);
+}
+// The last block of a cut unit whose first step is the line's `first`.
+FAV4_HD int last_block(int64_t first, int n, int64_t per, int slack) {
+  return static_cast<int>(quotient(first + n - 1 - slack, per));
+}
+
 }  // namespace fav4

@@ -474,6 +474,9 @@ __global__ void __launch_bounds__(384, 1)
         mbar_arrive(bar(L::kPieceFull + s));  // releases the writes above
         ++out;
       };
+      // 16 sequences of drafted tokens: 26.9 -> 26.1 us; a step of two Q tiles outweighs a piece (3 ragged chunks:
+      // 36.2 -> 38.6)
+      const int slack = QTiles == 1 ? piece_slack(per) : 0;
       if (begin < end) {
         int64_t base = scan[12], pos = begin;
         int b = static_cast<int>(scan[13]);
@@ -499,21 +502,20 @@ __global__ void __launch_bounds__(384, 1)
             }
             if (lane == 0) {
               int64_t first = base + h * head_work + before;  // the unit's place on the line
-              for (int64_t at = pos; at < stop && ok;) {
+              while (first < stop && ok) {
                 Piece w;
                 w.n = unit_steps(s, p.causal, bt, r);
+                w.tile0 = snap(begin - first, w.n, slack);
+                w.cnt = snap(end - first, w.n, slack) - w.tile0;
                 w.token0 = s.q0 + r * bt;
                 w.tokens = min(bt, s.sq - r * bt);
                 w.past = s.len - s.sq + r * bt;
                 w.len = s.len;
                 w.h = h;
                 w.b = b;
-                w.tile0 = static_cast<int>(at - first);
-                w.cnt = static_cast<int>(min(static_cast<int64_t>(w.n - w.tile0), end - at));
-                put(w);
-                if (w.tile0 == 0 && w.cnt < w.n)
-                  cut = make_int4(w.token0, w.tokens, h, static_cast<int>(quotient(first + w.n - 1, per)));
-                at += w.cnt;
+                if (w.cnt > 0) put(w);
+                if (w.tile0 == 0 && w.cnt > 0 && w.cnt < w.n)
+                  cut = make_int4(w.token0, w.tokens, h, last_block(first, w.n, per, slack));
                 first += w.n;
                 if (++r == units) {
                   r = 0;

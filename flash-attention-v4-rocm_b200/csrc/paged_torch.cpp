@@ -2,7 +2,7 @@
 //
 // A decode step calls these a few times per layer on work that takes the GPU a few microseconds, so the
 // host's share is kept small: arguments are read and checked here rather than in Python (a call costs the
-// host about 6 us, of which the launches are half, against 25 us through ctypes).
+// host about 4 us, of which the launch is half, against 25 us through ctypes).
 //
 // Workspaces: one for each device and stream, allocated from torch, its counters zeroed once, and kept; a
 // call that is being captured into a CUDA graph gets one of the graph's own memory with a captured zeroing,

@@ -37,6 +37,26 @@ int main() {
     }
     if (tile_seq_work(s, causal, bt) != sum) return 3;
   }
+  // units on a line, cut into stretches: every step is taken once, in order, by consecutive blocks
+  for (int it = 0; it < 20000; ++it) {
+    const int per = 1 + rand() % (it % 4 ? 9 : 60), slack = it % 3 ? piece_slack(per) : 0;
+    long first = rand() % 50;
+    for (int u = 0; u < 10; ++u) {
+      const int n = 1 + rand() % (it % 5 ? 12 : 200), c0 = (int)((first + slack) / per);
+      int done = 0, opened = -1, last = -1;
+      for (long c = first / per - 3 > 0 ? first / per - 3 : 0; c * per < first + n + 3 * per; ++c) {
+        const int from = snap(c * per - first, n, slack), to = snap((c + 1) * per - first, n, slack);
+        if (to <= from) continue;
+        if (from != done || (last >= 0 && c != last + 1)) return 5;
+        if (from == 0) opened = (int)c;
+        done = to;
+        last = (int)c;
+      }
+      if (done != n || opened < 0) return 6;
+      if (last != opened && (opened != c0 || last != last_block(first, n, per, slack))) return 7;
+      first += n;
+    }
+  }
   if (quotient(1L << 40, 3) != (1L << 40) / 3 || quotient(7, 1L << 33) != 0 || quotient(4294967295L, 2) != 2147483647L) return 4;
   printf("%ld\n", checked);
   return 0;
@@ -49,5 +69,5 @@ def test_closed_forms(tmp_path):
     src.write_text(PROGRAM)
     subprocess.run(["g++", "-O1", "-std=c++17", f"-I{F.PKG_ROOT / 'csrc'}", str(src), "-o", str(exe)], check=True)
     r = subprocess.run([str(exe)], capture_output=True, text=True)
-    assert r.returncode == 0, r.stdout
+    assert r.returncode == 0, (r.returncode, r.stdout)
     assert int(r.stdout) > 100000
