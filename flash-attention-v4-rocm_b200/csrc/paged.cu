@@ -18,6 +18,7 @@ namespace {
 
 constexpr int kMaxDevices = 64;
 constexpr int kMaxSms = 160;         // bound on the SMs that the workspace is laid out for (a B200 has 148)
+constexpr long long kKeyMargin = 8192;  // the kernels' key indexes go this far past a sequence's length at most
 constexpr int kPagedPerSm = 2;       // blocks of paged_attn_kernel per SM
 constexpr int kMaxGrid = kMaxSms * kPagedPerSm;
 
@@ -74,7 +75,7 @@ bool cache_valid(const Fav4PagedCache& c) {
          aligned4(c.seq_lens) && stride_ok(c.page_stride) && stride_ok(c.token_stride) && stride_ok(c.head_stride) &&
          c.batch > 0 && c.batch < INT_MAX && c.kv_heads > 0 && c.num_pages > 0 && c.page_size >= 16 &&
          c.page_size % 16 == 0 && c.max_pages > 0 && c.table_stride >= 0 &&
-         static_cast<long long>(c.max_pages) * c.page_size <= INT_MAX - 1024;
+         static_cast<long long>(c.max_pages) * c.page_size <= INT_MAX - kKeyMargin;
 }
 
 PagedCacheView view_of(const Fav4PagedCache& c) {
@@ -118,7 +119,7 @@ bool paged_valid(const Fav4PagedArgs* a) {
     return false;
   if (a->prefix_pages &&
       (!aligned4(a->prefix_pages) || !aligned4(a->prefix_len) || a->max_prefix_pages <= 0 ||
-       static_cast<long long>(a->max_prefix_pages) * a->cache.page_size > INT_MAX - 1024))
+       static_cast<long long>(a->max_prefix_pages) * a->cache.page_size > INT_MAX - kKeyMargin))
     return false;
   if (a->total_q == 0) return true;
   return a->max_sq > 0 && a->q && a->o && aligned16(a->q) && aligned16(a->o) && aligned4(a->lse) &&

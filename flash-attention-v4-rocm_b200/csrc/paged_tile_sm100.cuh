@@ -276,7 +276,7 @@ __global__ void __launch_bounds__(384, 1)
         // lane x < groups has the page of keys [128 j + x R, + R) of the next tile j
         const int* table = p.c.table + w.b * p.c.table_stride;
         auto page_of = [&](int j) -> int {
-          const int key = (w.tile0 + j) * kTileKeys + lane * R;  // lengths stay 1024 below INT_MAX
+          const int key = (w.tile0 + j) * kTileKeys + lane * R;  // lengths stay well below INT_MAX
           if (lane >= groups || j >= N || key >= w.len) return 0;
           return min(max(__ldg(table + key / p.c.page_size), 0), p.c.num_pages - 1);
         };

@@ -13,6 +13,7 @@ build/fav4_paged_torch.so is the PyTorch binding of the paged cache entries
 from __future__ import annotations
 
 import argparse
+import importlib.util
 import os
 import shutil
 import subprocess
@@ -63,17 +64,17 @@ def binding_command(out: Path) -> list[str]:
     import sysconfig
 
     import torch
-    from torch.utils import cpp_extension
 
-    home = Path(nvcc()).resolve().parents[1]
-    includes = [*cpp_extension.include_paths(), str(home / "include"), sysconfig.get_paths()["include"], str(INCLUDE)]
-    libs = Path(torch.__file__).parent / "lib"
+    home, lib = Path(nvcc()).resolve().parents[1], Path(torch.__file__).parent
+    includes = [lib / "include", lib / "include" / "torch" / "csrc" / "api" / "include", home / "include",
+                sysconfig.get_paths()["include"], INCLUDE]
     cxx = os.environ.get("CXX") or shutil.which("g++") or "c++"
-    # the C++ runtime that torch itself runs on, never a static copy of the compiler's
-    return [cxx, "-O2", "-std=c++17", "-fPIC", "-shared", "-nostdlib++", f"-D_GLIBCXX_USE_CXX11_ABI={int(torch.compiled_with_cxx11_abi())}",
-            *[f"-isystem{i}" for i in includes], str(BINDING_SRC), "-o", str(out), f"-L{BUILD}", f"-L{libs}",
-            "-l:libfav4_bshd.so", "-lc10", "-lc10_cuda", "-ltorch_cpu", "-ltorch_python",
-            f"-L{home / 'lib64'}", "-lcudart", "-l:libstdc++.so.6", "-Wl,-rpath,$ORIGIN", f"-Wl,-rpath,{libs}"]
+    # -nostdlib++ and libstdc++.so: the C++ runtime that torch itself runs on, never a static copy of the compiler's
+    return [cxx, "-O2", "-std=c++17", "-fPIC", "-shared", "-nostdlib++",
+            f"-D_GLIBCXX_USE_CXX11_ABI={int(torch.compiled_with_cxx11_abi())}", *[f"-isystem{i}" for i in includes],
+            str(BINDING_SRC), "-o", str(out), f"-L{BUILD}", f"-L{lib / 'lib'}", f"-L{home / 'lib64'}",
+            "-l:libfav4_bshd.so", "-lc10", "-lc10_cuda", "-ltorch_cpu", "-ltorch_python", "-lcudart",
+            "-l:libstdc++.so.6", "-Wl,-rpath,$ORIGIN", f"-Wl,-rpath,{lib / 'lib'}"]
 
 
 def build(force: bool = False, verbose: bool = False) -> list[Path]:
@@ -87,6 +88,9 @@ def build(force: bool = False, verbose: bool = False) -> list[Path]:
             _run(cmd, BUILD / f"{lib}.ptxas.txt", lib, verbose)
         built.append(out)
     out = BUILD / BINDING
+    if importlib.util.find_spec("torch") is None:
+        print(f"{BINDING} is not built: there is no torch here (the C ABI does not need it)", file=sys.stderr)
+        return built
     if force or _stale(out, [BINDING_SRC, *INCLUDE.glob("*.h")]):
         _run(binding_command(out), BUILD / f"{BINDING}.log", BINDING, verbose)
     return [*built, out]

@@ -25,8 +25,8 @@ BINDING_PATH = BUILD_DIR / "fav4_paged_torch.so"
 _BINDING = None
 
 
-def _binding():
-    """The native module that checks the arguments and calls the library (csrc/paged_torch.cpp)."""
+def load_binding():
+    """Load (once) the native module that checks the arguments and calls the library (csrc/paged_torch.cpp)."""
     global _BINDING
     if _BINDING is None:
         if not BINDING_PATH.exists():
@@ -47,7 +47,7 @@ def append(q, k, v, k_cache, v_cache, page_table, seq_lens, cu_q, cos=None, sin=
     (FP32 ``[positions, rotary/2]``) at their positions; ``cos=None`` appends without rotation. q ``[T, H, 128]``, k and
     v ``[T, H_kv, 128]`` may be strided (slices of one projection). ``offsets`` (int32 ``[B]``) shifts a sequence's
     rotation positions, for keys behind a shared prefix. ``out`` may be q's own memory when q is contiguous."""
-    return _binding().append(q, k, v, k_cache, v_cache, page_table, seq_lens, cu_q, cos, sin, interleaved, offsets, out)
+    return load_binding().append(q, k, v, k_cache, v_cache, page_table, seq_lens, cu_q, cos, sin, interleaved, offsets, out)
 
 
 def attention(q, k_cache, v_cache, page_table, seq_lens, cu_q, max_sq: int, *, causal=True, scale=None, out=None,
@@ -55,7 +55,7 @@ def attention(q, k_cache, v_cache, page_table, seq_lens, cu_q, max_sq: int, *, c
     """O ``[T, H, 128]``, or (O, LSE ``[H, T]``), of packed queries over the pages. ``max_sq`` bounds the new tokens of
     a sequence. Causal is bottom-right: row i of sq sees keys up to ``seq_lens[b] - sq + i``; rows without a key get
     O = 0 and LSE = -inf."""
-    return _binding().attend(q, k_cache, v_cache, page_table, seq_lens, cu_q, max_sq, causal, scale, out, return_lse,
+    return load_binding().attend(q, k_cache, v_cache, page_table, seq_lens, cu_q, max_sq, causal, scale, out, return_lse,
                              None, None)
 
 
@@ -64,8 +64,8 @@ def shared_prefix_attention(q, k_cache, v_cache, prefix_pages, prefix_len, page_
     """``attention`` where ``prefix_len`` (device int32 ``[1]``) keys at ``prefix_pages`` (device int32 ``[n]``) stand
     before every sequence's own keys and are read once for the whole batch; ``seq_lens`` and ``page_table`` are the
     sequences' own."""
-    return _binding().attend(q, k_cache, v_cache, page_table, seq_lens, cu_q, max_sq, causal, scale, out, return_lse,
+    return load_binding().attend(q, k_cache, v_cache, page_table, seq_lens, cu_q, max_sq, causal, scale, out, return_lse,
                              prefix_pages, prefix_len)
 
 
-__all__ = ["HEAD_DIM", "BINDING_PATH", "append", "attention", "shared_prefix_attention"]
+__all__ = ["HEAD_DIM", "BINDING_PATH", "load_binding", "append", "attention", "shared_prefix_attention"]
