@@ -40,6 +40,12 @@ SHAPES = [
     ([40, 1], [600, 64], 7, 1, 16),                  # a group of 7
     ([5, 70], [300, 333], 160, 1, 32),               # more query heads per K/V head than a tile has rows
     ([512], [4000], 8, 8, 256),
+    # two tiles per block
+    ([700, 1000, 850], [700, 2387, 1500], 6, 3, 48),
+    ([2100, 1], [2100, 900], 8, 8, 64),
+    ([513, 30], [1700, 30], 8, 2, 16),
+    ([700, 5, 90], [690, 3, 1000], 12, 4, 32),       # a group of 3, rows before the first key
+    ([129, 600], [0, 777], 40, 2, 16),               # a group of 20; a sequence without keys
 ]
 
 
@@ -72,6 +78,8 @@ PREFIXED = [
     ([3, 2], [1, 0], 4, 2, 16, 0),                    # no prefix keys: empty rows stay empty
     ([200, 100], [200, 150], 8, 2, 64, 777),
     ([9], [20], 160, 1, 16, 333),
+    ([300, 260], [300, 700], 8, 2, 64, 1500),        # two tiles per block for the prefix
+    ([9] * 30, [9 + 7 * i for i in range(30)], 8, 1, 16, 2500),
 ]
 
 
