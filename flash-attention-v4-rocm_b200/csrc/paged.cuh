@@ -325,7 +325,7 @@ __device__ __forceinline__ bool row_place(const PagedParams& p, const SeqView& s
 }
 
 // One finished row: columns 4 lane .. 4 lane + 3 of sum / l, joined with the other result if there is one.
-__device__ __noinline__ void finish_row(const PagedParams& p, const RowPlace& at, float4 acc, float m, float l,
+__device__ __forceinline__ void finish_row(const PagedParams& p, const RowPlace& at, float4 acc, float m, float l,
                                            int lane) {
   const int64_t row = static_cast<int64_t>(at.token) * p.heads + at.head;
   const int64_t lse_at = static_cast<int64_t>(at.head) * p.total_q + at.token;
