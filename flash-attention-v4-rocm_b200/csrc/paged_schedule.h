@@ -62,7 +62,7 @@ FAV4_HD int unit_steps(const SeqView& s, int causal, int bt, int r) {
   const int64_t last = full < s.sq ? full : s.sq;
   return steps_up_to(causal ? static_cast<int64_t>(s.len) - s.sq + last : s.len);
 }
-FAV4_HD_CALL int64_t units_steps(const SeqView& s, int causal, int bt, int64_t r) {
+FAV4_HD_CALL int64_t units_steps(SeqView s, int causal, int bt, int64_t r) {
   if (r <= 0) return 0;
   if (!causal) return r * steps_up_to(s.len);
   const int64_t units = quotient(static_cast<int64_t>(s.sq) + bt - 1, bt);
