@@ -86,8 +86,10 @@ FAV4_HD int64_t tile_seq_work(const SeqView& s, int causal, int bt) {
 // long that the imbalance would cost more than the piece.
 FAV4_HD int piece_slack(int64_t per) { return per > 32 ? 0 : static_cast<int>(per / 4 < 2 ? per / 4 : 2); }
 // Where a boundary between two blocks, `at` steps into a unit of n, really cuts: at its begin or end if that is
-// at most `slack` steps away. Both blocks ask, so what one leaves the other takes.
+// at most `slack` steps away; one that is not inside the unit cuts nothing off it. Both blocks ask, so what one
+// leaves the other takes.
 FAV4_HD int snap(int64_t at, int n, int slack) {
+  if (at >= n) return n;
   if (at <= slack) return 0;
   return at >= n - slack ? n : static_cast<int>(at);
 }

@@ -40,6 +40,10 @@ SHAPES = [
     ([40, 1], [600, 64], 7, 1, 16),                  # a group of 7
     ([5, 70], [300, 333], 160, 1, 32),               # more query heads per K/V head than a tile has rows
     ([512], [4000], 8, 8, 256),
+    # chunks among sequences of a key or none, whose units of one step lie at the blocks' boundaries
+    ([1, 0, 121, 14, 1, 77, 383, 2, 1, 1, 0, 2, 1, 2, 348, 0, 2, 209, 1, 1, 473, 2, 1, 461, 1, 369, 2, 2, 1, 0, 1, 0, 1],
+     [786, 10, 846, 324, 497, 354, 815, 453, 0, 706, 540, 277, 933, 525, 650, 834, 759, 385, 626, 987, 1149, 2, 956, 655,
+      892, 1304, 970, 143, 452, 246, 698, 406, 979], 3, 3, 32),
     # two tiles per block
     ([700, 1000, 850], [700, 2387, 1500], 6, 3, 48),
     ([2100, 1], [2100, 900], 8, 8, 64),

@@ -37,24 +37,33 @@ int main() {
     }
     if (tile_seq_work(s, causal, bt) != sum) return 3;
   }
-  // units on a line, cut into stretches: every step is taken once, in order, by consecutive blocks
+  // units on a line, cut into stretches as the blocks do it, each from the unit that holds its begin to the last
+  // one that begins before its end: every step is taken once, in order, by consecutive blocks
   for (int it = 0; it < 20000; ++it) {
-    const int per = 1 + rand() % (it % 4 ? 9 : 60), slack = it % 3 ? piece_slack(per) : 0;
-    long first = rand() % 50;
-    for (int u = 0; u < 10; ++u) {
-      const int n = 1 + rand() % (it % 5 ? 12 : 200), c0 = (int)((first + slack) / per);
-      int done = 0, opened = -1, last = -1;
-      for (long c = first / per - 3 > 0 ? first / per - 3 : 0; c * per < first + n + 3 * per; ++c) {
-        const int from = snap(c * per - first, n, slack), to = snap((c + 1) * per - first, n, slack);
+    const int per = 1 + rand() % (it % 4 ? 9 : 60), slack = it % 3 ? piece_slack(per) : 0, units = 1 + rand() % 12;
+    long first[13] = {0};
+    int n[12], done[12] = {0}, opened[12], last[12];
+    for (int u = 0; u < units; ++u) {
+      n[u] = 1 + rand() % (it % 5 ? 12 : 200);
+      if (it % 2 && rand() % 2) n[u] = 1;
+      first[u + 1] = first[u] + n[u];
+      opened[u] = last[u] = -1;
+    }
+    for (long c = 0; c * per < first[units]; ++c) {
+      const long begin = c * per, end = begin + per < first[units] ? begin + per : first[units];
+      for (int u = 0; u < units; ++u) {
+        if (first[u + 1] <= begin || first[u] >= end) continue;
+        const int from = snap(begin - first[u], n[u], slack), to = snap(end - first[u], n[u], slack);
         if (to <= from) continue;
-        if (from != done || (last >= 0 && c != last + 1)) return 5;
-        if (from == 0) opened = (int)c;
-        done = to;
-        last = (int)c;
+        if (from != done[u] || (last[u] >= 0 && c != last[u] + 1)) return 5;
+        if (from == 0) opened[u] = (int)c;
+        done[u] = to;
+        last[u] = (int)c;
       }
-      if (done != n || opened < 0) return 6;
-      if (last != opened && (opened != c0 || last != last_block(first, n, per, slack))) return 7;
-      first += n;
+    }
+    for (int u = 0; u < units; ++u) {
+      if (done[u] != n[u] || opened[u] < 0) return 6;
+      if (last[u] != opened[u] && last[u] != last_block(first[u], n[u], per, slack)) return 7;
     }
   }
   if (quotient(1L << 40, 3) != (1L << 40) / 3 || quotient(7, 1L << 33) != 0 || quotient(4294967295L, 2) != 2147483647L) return 4;
