@@ -17,8 +17,8 @@
 //   warp 11          the schedule: pieces of work into a small ring that the other warps read
 //
 // Schedule. A unit is (sequence, K/V head, Q tiles of `block_tokens` tokens) and has as many steps as
-// 128-key tiles up to its last visible key. All units lie on one line of steps and every block takes an
-// equal stretch of it, so ragged batches, causal chunks and few rows against many keys are balanced
+// 128-key tiles up to its last visible key. All units lie on one line of steps, with room before each for what
+// it costs beside them, and every block takes an equal stretch of it, so ragged batches, causal chunks and few rows against many keys are balanced
 // alike; the prefix sums of the steps have a closed form, so the line needs no plan and no host. A unit
 // that a boundary cuts leaves (m, l, O) per piece in the workspace, in FP32, and paged_join_kernel adds
 // them up in key order.
@@ -474,9 +474,6 @@ __global__ void __launch_bounds__(384, 1)
         mbar_arrive(bar(L::kPieceFull + s));  // releases the writes above
         ++out;
       };
-      // 16 sequences of drafted tokens: 26.9 -> 26.1 us; a step of two Q tiles outweighs a piece (3 ragged chunks:
-      // 36.2 -> 38.6)
-      const int slack = QTiles == 1 ? piece_slack(per) : 0;
       if (begin < end) {
         int64_t base = scan[12], pos = begin;
         int b = static_cast<int>(scan[13]);
@@ -490,11 +487,11 @@ __global__ void __launch_bounds__(384, 1)
             // the unit that holds `pos`: the last r whose earlier units end at or before it, 32 probes a round
             const int64_t x = pos - base - h * head_work;
             int r = 0, hi = units;  // r fits, hi does not
-            int64_t before = 0;     // steps of the units before r
+            int64_t before = 0;     // cost of the units before r
             while (hi - r > 1) {
               const int step = (hi - r + 31) / 32;
               const int64_t probe = r + static_cast<int64_t>(lane) * step;
-              const int64_t sum = probe < hi ? units_steps(s, p.causal, bt, probe) : 0;
+              const int64_t sum = probe < hi ? units_cost(s, p.causal, bt, probe) : 0;
               const int n = __popc(__ballot_sync(0xffffffffu, probe < hi && sum <= x));  // lane 0 always fits
               before = __shfl_sync(0xffffffffu, sum, n - 1);
               r += (n - 1) * step;
@@ -505,8 +502,9 @@ __global__ void __launch_bounds__(384, 1)
               while (first < stop && ok) {
                 Piece w;
                 w.n = unit_steps(s, p.causal, bt, r);
-                w.tile0 = snap(begin - first, w.n, slack);
-                w.cnt = snap(end - first, w.n, slack) - w.tile0;
+                const int64_t step0 = first + kUnitExtra;  // the place of its first step
+                w.tile0 = steps_before(begin - step0, w.n);
+                w.cnt = steps_before(end - step0, w.n) - w.tile0;
                 w.token0 = s.q0 + r * bt;
                 w.tokens = min(bt, s.sq - r * bt);
                 w.past = s.len - s.sq + r * bt;
@@ -515,8 +513,8 @@ __global__ void __launch_bounds__(384, 1)
                 w.b = b;
                 if (w.cnt > 0) put(w);
                 if (w.tile0 == 0 && w.cnt > 0 && w.cnt < w.n)
-                  cut = make_int4(w.token0, w.tokens, h, last_block(first, w.n, per, slack));
-                first += w.n;
+                  cut = make_int4(w.token0, w.tokens, h, static_cast<int>(quotient(step0 + w.n - 1, per)));
+                first = step0 + w.n;
                 if (++r == units) {
                   r = 0;
                   ++h;

@@ -35,25 +35,26 @@ int main() {
       if (unit_steps(s, causal, bt, r) != want) return 2;
       sum += want;
     }
-    if (tile_seq_work(s, causal, bt) != sum) return 3;
+    if (tile_seq_work(s, causal, bt) != sum + kUnitExtra * units) return 3;
   }
   // units on a line, cut into stretches as the blocks do it, each from the unit that holds its begin to the last
   // one that begins before its end: every step is taken once, in order, by consecutive blocks
   for (int it = 0; it < 20000; ++it) {
-    const int per = 1 + rand() % (it % 4 ? 9 : 60), slack = it % 3 ? piece_slack(per) : 0, units = 1 + rand() % 12;
+    const int per = 1 + rand() % (it % 4 ? 9 : 60), units = 1 + rand() % 12;
     long first[13] = {0};
     int n[12], done[12] = {0}, opened[12], last[12];
     for (int u = 0; u < units; ++u) {
       n[u] = 1 + rand() % (it % 5 ? 12 : 200);
       if (it % 2 && rand() % 2) n[u] = 1;
-      first[u + 1] = first[u] + n[u];
+      first[u + 1] = first[u] + kUnitExtra + n[u];
       opened[u] = last[u] = -1;
     }
     for (long c = 0; c * per < first[units]; ++c) {
       const long begin = c * per, end = begin + per < first[units] ? begin + per : first[units];
       for (int u = 0; u < units; ++u) {
         if (first[u + 1] <= begin || first[u] >= end) continue;
-        const int from = snap(begin - first[u], n[u], slack), to = snap(end - first[u], n[u], slack);
+        const long step0 = first[u] + kUnitExtra;
+        const int from = steps_before(begin - step0, n[u]), to = steps_before(end - step0, n[u]);
         if (to <= from) continue;
         if (from != done[u] || (last[u] >= 0 && c != last[u] + 1)) return 5;
         if (from == 0) opened[u] = (int)c;
@@ -62,8 +63,8 @@ int main() {
       }
     }
     for (int u = 0; u < units; ++u) {
-      if (done[u] != n[u] || opened[u] < 0) return 6;
-      if (last[u] != opened[u] && last[u] != last_block(first[u], n[u], per, slack)) return 7;
+      const long step0 = first[u] + kUnitExtra;
+      if (done[u] != n[u] || opened[u] != step0 / per || last[u] != (step0 + n[u] - 1) / per) return 6;
     }
   }
   if (quotient(1L << 40, 3) != (1L << 40) / 3 || quotient(7, 1L << 33) != 0 || quotient(4294967295L, 2) != 2147483647L) return 4;
