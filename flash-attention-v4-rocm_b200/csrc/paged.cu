@@ -127,23 +127,24 @@ bool paged_valid(const Fav4PagedArgs* a) {
          stride_ok(a->q_token_stride) && stride_ok(a->q_head_stride);
 }
 
-// Q tiles per block for `batch` sequences of at most `tokens` new tokens each, `total` in all; 0 for
-// paged_attn_kernel. `rows` of a sequence share a K/V head; lengths are not known here.
+// Q tiles per block for `batch` sequences of at most `tokens` new tokens each behind page tables for `capacity`
+// keys; 0 for paged_attn_kernel. `rows` of a sequence share a K/V head; lengths are not known here.
 //   16-row kernel or tiles. Up to 16 rows the former reads at HBM speed with half the start-up: 32 sequences
-//   of up to 32767 keys take 91 us against 106 with 4 rows, 62 against 62 with 16 (and with 24: 82 against 61).
+//   of up to 32767 keys take 89 us against 103 with 4 rows, 58 against 62 with 16 (and with 24: 79 against 62).
 //   But the last block of a unit joins its pieces alone, and with few units there are many: with 8 rows, one
-//   unit of 8000 keys 27 us against 16, four units 22 against 18, eight 21 against 20, 64 units of 500 to 1500
-//   keys 21 against 24. With 16 rows 16 units of 100 to 1000 keys 20 against 17, 32 of 8000 38 against 44.
-//   One tile or two. Two tiles read each key half as often and hide one tile's softmax behind the other's
-//   products: 4 x 4096 tokens 187 us against 255, 3 ragged chunks (up to 2000 rows) 36 against 46. One tile
-//   makes smaller pieces and less padding where the blocks are not full anyway: 8 x 257 rows of 8 heads 23
-//   against 29, 384 rows behind 4000 keys 21 against 23, 1024 rows x 8 units 31 against 32; one sequence of
-//   2048 rows 46 against 43.
-int q_tiles(long long tokens, long long total, int batch, int group, int kv_heads) {
+//   unit of 8000 keys 27 us against 17, four units 20 against 17, eight 18 against 19, 64 units of 500 to 1500
+//   keys 15 against 21. With 16 rows 16 units of 100 to 1000 keys 15 against 14, 32 of 8000 34 against 39.
+//   One tile or two. Two tiles read each key half as often and have half the units; one makes smaller pieces and
+//   less padding and has both warpgroups on every step. Long chunks take two: 4096 tokens behind 28672 keys (16384
+//   rows) 502 us against 525, 3 ragged ones of up to 2000 rows 31 against 33, 8 of 1024 rows behind 8000 keys 87
+//   against 93 (but one of 2048 rows behind 8000 35 against 33); and so do prompts that begin their sequence, whose
+//   units have few steps, as tables not much wider than the chunk tell: 4 of 4096 tokens 171 against 183, 8 of 512
+//   rows (8 heads) 23 against 32, 8 of 257 24 against 26. The others take one: 32 of 600 rows behind 1000 keys 49
+//   against 55, 4 of 600 (8 heads) behind 600 32 against 39, 256 rows on 32768 keys 27 against 32.
+int q_tiles(long long tokens, int batch, int group, int kv_heads, long long capacity) {
   const long long rows = tokens * group, units = static_cast<long long>(batch) * kv_heads;
   if (group > kBlockM || (rows <= kPagedRows && rows < 2 * units && (rows <= 8 || units >= 32))) return 0;
-  const long long tiles = total * group * kv_heads / kBlockM;
-  return rows > 512 && (tiles >= 96 || rows >= 2048) ? 2 : 1;
+  return rows >= 1024 || (rows > kBlockM && capacity < 2 * tokens) ? 2 : 1;
 }
 
 // Workspace: counters first (their place never changes, so that any call may follow any other), then the
@@ -159,8 +160,10 @@ static_assert(2 * kMaxGrid * sizeof(uint32_t) <= PagedSpace::kCounters, "two cal
 static_assert(kMaxSms <= 256, "paged_join_kernel reads one cut unit per thread");
 PagedSpace paged_space(const Fav4PagedArgs& a) {
   const int group = a.heads / a.cache.kv_heads;
-  int tiles = q_tiles(a.max_sq, a.total_q, a.cache.batch, group, a.cache.kv_heads);
-  if (a.prefix_pages) tiles = std::max(tiles, q_tiles(a.total_q, a.total_q, 1, group, a.cache.kv_heads));
+  const long long page = a.cache.page_size;
+  int tiles = q_tiles(a.max_sq, a.cache.batch, group, a.cache.kv_heads, a.cache.max_pages * page);
+  if (a.prefix_pages)
+    tiles = std::max(tiles, q_tiles(a.total_q, 1, group, a.cache.kv_heads, a.max_prefix_pages * page));
   PagedSpace s;
   s.part = PagedSpace::kCounters;
   s.tile_o = s.part + (a.prefix_pages ? 2 : 1) * PagedSpace::kPart;
@@ -214,7 +217,8 @@ int launch_rows(const PagedParams& p, const PagedSpace& sp, uint8_t* ws, int sms
   // a cache expanded over heads or pages (stride 0) has no tensor map
   const bool mapped = (p.c.head_stride > 0 || p.c.kv_heads == 1) && (p.c.page_stride > 0 || p.c.num_pages == 1) &&
                       p.c.token_stride > 0 && (p.q_hs > 0 || p.heads == 1) && (p.q_ts > 0 || p.total_q == 1);
-  const int tiles = mapped ? q_tiles(p.max_sq, p.total_q, p.c.batch, p.group, p.c.kv_heads) : 0;
+  const long long capacity = static_cast<long long>(p.c.max_pages) * p.c.page_size;
+  const int tiles = mapped ? q_tiles(p.max_sq, p.c.batch, p.group, p.c.kv_heads, capacity) : 0;
   if (tiles == 1) return launch_tiles<1>(p, sp, ws, sms, stream);
   if (tiles == 2) return launch_tiles<2>(p, sp, ws, sms, stream);
   return launch(p.add_o ? paged_attn_kernel<true> : paged_attn_kernel<false>, sms * kPagedPerSm, kPagedWarps * 32, kPagedSmem, stream, p);
