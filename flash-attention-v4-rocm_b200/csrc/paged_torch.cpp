@@ -18,6 +18,8 @@
 
 #include <climits>
 #include <cmath>
+#include <cstdint>
+#include <initializer_list>
 #include <map>
 #include <utility>
 
@@ -69,9 +71,18 @@ const void* rows(const at::Tensor& t, const char* name, const at::Device& dev, i
   *head_stride = t.size(1) > 1 ? t.stride(1) : 0;
   return t.const_data_ptr();
 }
-void no_grad(const at::Tensor& t, const char* what) {
-  TORCH_CHECK(!(t.requires_grad() && at::GradMode::is_enabled()), what,
-              " has no gradient: call it under torch.no_grad(), or detach its inputs");
+void no_grad(const char* what, std::initializer_list<const at::Tensor*> tensors) {
+  if (!at::GradMode::is_enabled()) return;
+  for (const at::Tensor* t : tensors)
+    TORCH_CHECK(!t->requires_grad(), what, " has no gradient: call it under torch.no_grad(), or detach its inputs");
+}
+// Whether a contiguous result and an input share memory: other blocks still read rows where one writes its own.
+bool overlap(const at::Tensor& out, const at::Tensor& in) {
+  if (out.numel() == 0 || in.numel() == 0) return false;
+  int64_t last = 0;
+  for (int64_t d = 0; d < in.dim(); ++d) last += (in.size(d) - 1) * in.stride(d);
+  const auto o = reinterpret_cast<uintptr_t>(out.const_data_ptr()), i = reinterpret_cast<uintptr_t>(in.const_data_ptr());
+  return o < i + (last + 1) * in.element_size() && i < o + out.numel() * out.element_size();
 }
 
 Fav4PagedCache cache_of(PyObject* const* a, const at::Device& dev) {
@@ -132,9 +143,7 @@ PyObject* append(PyObject*, PyObject* const* a, Py_ssize_t n) {
   const at::Tensor& v = tensor_arg(a[2], "v");
   const at::Device dev = q.device();
   TORCH_CHECK(dev.is_cuda(), "q must be on a CUDA device, got ", dev);
-  no_grad(q, "append");
-  no_grad(k, "append");
-  no_grad(v, "append");
+  no_grad("append", {&q, &k, &v, &tensor_arg(a[3], "k_cache"), &tensor_arg(a[4], "v_cache")});
   const c10::cuda::CUDAGuard guard(dev);
   Fav4PagedAppendArgs p = {};
   p.cache = cache_of(a + 3, dev);
@@ -147,6 +156,7 @@ PyObject* append(PyObject*, PyObject* const* a, Py_ssize_t n) {
   if (a[8] != Py_None) {
     const at::Tensor& c = tensor_arg(a[8], "cos");
     const at::Tensor& s = tensor_arg(a[9], "sin");
+    no_grad("append", {&c, &s});
     TORCH_CHECK(c.dim() == 2 && s.sizes() == c.sizes() && c.is_contiguous() && s.is_contiguous() &&
                     c.scalar_type() == at::kFloat && s.scalar_type() == at::kFloat && c.device() == dev &&
                     s.device() == dev && c.size(1) >= 8 && c.size(1) % 8 == 0 && c.size(1) <= kHeadDim / 2,
@@ -166,6 +176,11 @@ PyObject* append(PyObject*, PyObject* const* a, Py_ssize_t n) {
     out = tensor_arg(a[12], "out");
     TORCH_CHECK(out.sizes() == q.sizes() && out.scalar_type() == at::kBFloat16 && out.device() == dev && out.is_contiguous(),
                 "out must be contiguous bfloat16 of q's shape");
+    no_grad("append", {&out});
+    // a row of q may be turned in its own place
+    TORCH_CHECK((q.is_contiguous() && out.const_data_ptr() == q.const_data_ptr()) || !overlap(out, q),
+                "out may be q's own memory, but not a part of it");
+    TORCH_CHECK(!overlap(out, k) && !overlap(out, v), "out must not overlap k or v");
   }
   p.q_out = out.data_ptr();
   p.heads = fits(heads, "heads");
@@ -183,7 +198,7 @@ PyObject* attend(PyObject*, PyObject* const* a, Py_ssize_t n) {
   const at::Tensor& q = tensor_arg(a[0], "q");
   const at::Device dev = q.device();
   TORCH_CHECK(dev.is_cuda(), "q must be on a CUDA device, got ", dev);
-  no_grad(q, "paged attention");
+  no_grad("paged attention", {&q, &tensor_arg(a[1], "k_cache"), &tensor_arg(a[2], "v_cache")});
   const c10::cuda::CUDAGuard guard(dev);
   Fav4PagedArgs p = {};
   p.cache = cache_of(a + 1, dev);
@@ -221,6 +236,8 @@ PyObject* attend(PyObject*, PyObject* const* a, Py_ssize_t n) {
     out = tensor_arg(a[9], "out");
     TORCH_CHECK(out.sizes() == q.sizes() && out.scalar_type() == at::kBFloat16 && out.device() == dev && out.is_contiguous(),
                 "out must be contiguous bfloat16 of q's shape");
+    no_grad("paged attention", {&out});
+    TORCH_CHECK(!overlap(out, q), "out must not overlap q");
   }
   p.o = out.data_ptr();
   const bool with_lse = bool_arg(a[10]);

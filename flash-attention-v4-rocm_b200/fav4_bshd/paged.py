@@ -54,7 +54,8 @@ def attention(q, k_cache, v_cache, page_table, seq_lens, cu_q, max_sq: int, *, c
               return_lse=False):
     """O ``[T, H, 128]``, or (O, LSE ``[H, T]``), of packed queries over the pages. ``max_sq`` bounds the new tokens of
     a sequence. Causal is bottom-right: row i of sq sees keys up to ``seq_lens[b] - sq + i``; rows without a key get
-    O = 0 and LSE = -inf."""
+    O = 0 and LSE = -inf. ``out`` must not overlap q. Rows of no sequence, and a sequence's rows past ``max_sq``, are
+    not written."""
     return load_binding().attend(q, k_cache, v_cache, page_table, seq_lens, cu_q, max_sq, causal, scale, out, return_lse,
                              None, None)
 

@@ -493,3 +493,37 @@ def test_offsets_past_32_bits(cuda, sq):
     at = torch.arange(n - sq, n, device=cuda)
     rows = table[0].long()[at // page]
     assert torch.equal(k_cache[rows, at % page], k) and torch.equal(v_cache[rows, at % page], -k)
+
+
+def test_every_input_that_wants_a_gradient_is_refused(cuda):
+    x = Batch([2, 1], [50, 40], 8, 2, 16, seed=61)
+    q, k, v, _, cos, sin = do_append(x, 128, False, cuda, fused=False)
+    wants = lambda t: t.clone().requires_grad_()
+    appends = [q, k, v, x.k_cache, x.v_cache, x.table, x.lens, x.cu, cos, sin]
+    for i in (0, 1, 2, 3, 4, 8, 9):
+        with pytest.raises(RuntimeError, match="no gradient"):
+            paged.append(*[wants(t) if j == i else t for j, t in enumerate(appends)])
+    attends = [x.q, x.k_cache, x.v_cache, x.table, x.lens, x.cu, 2]
+    for i in (0, 1, 2):
+        with pytest.raises(RuntimeError, match="no gradient"):
+            paged.attention(*[wants(t) if j == i else t for j, t in enumerate(attends)])
+    with pytest.raises(RuntimeError, match="no gradient"):
+        paged.attention(*attends, out=wants(x.q))
+
+
+def test_results_that_overlap_an_input_are_refused(cuda):
+    x = Batch([2, 1], [50, 40], 8, 2, 16, seed=62)
+    q, k, v, _, cos, sin = do_append(x, 128, False, cuda, fused=False)
+    cache = (x.k_cache, x.v_cache, x.table, x.lens, x.cu)
+    both = torch.zeros(4, 8, D, dtype=torch.bfloat16, device=cuda)
+    for out in (both[:3], both[1:]):
+        with pytest.raises(RuntimeError, match="overlap"):
+            paged.attention(both[:3], *cache, 2, out=out)
+    with pytest.raises(RuntimeError, match="not a part"):
+        paged.append(both[:3], k, v, *cache, cos, sin, out=both[1:])
+    wide = torch.zeros(3, 12, D, dtype=torch.bfloat16, device=cuda)  # out over a projection's slices
+    with pytest.raises(RuntimeError, match="not a part"):
+        paged.append(wide[:, :8], wide[:, 8:10], wide[:, 10:], *cache, cos, sin, out=wide.view(-1)[:3 * 8 * D].view(3, 8, D))
+    with pytest.raises(RuntimeError, match="overlap k or v"):
+        paged.append(q, both.view(-1)[:3 * 2 * D].view(3, 2, D), v, *cache, cos, sin, out=both[:3])
+    paged.attention(both[:3], *cache, 2, out=torch.empty_like(both[:3]))
