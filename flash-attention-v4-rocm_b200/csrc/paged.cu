@@ -212,16 +212,22 @@ int launch_tiles(const PagedParams& p, const PagedSpace& sp, uint8_t* ws, int sm
   return launch(paged_join_kernel<QTiles>, kJoinPerSm * sms, 256, 0, stream, t, sms);
 }
 
-// One attention of all rows over one set of page tables.
-int launch_rows(const PagedParams& p, const PagedSpace& sp, uint8_t* ws, int sms, cudaStream_t stream) {
+long long key_capacity(const PagedParams& p) { return static_cast<long long>(p.c.max_pages) * p.c.page_size; }
+
+int tiles_of(const PagedParams& p) {
   // a cache expanded over heads or pages (stride 0) has no tensor map
   const bool mapped = (p.c.head_stride > 0 || p.c.kv_heads == 1) && (p.c.page_stride > 0 || p.c.num_pages == 1) &&
                       p.c.token_stride > 0 && (p.q_hs > 0 || p.heads == 1) && (p.q_ts > 0 || p.total_q == 1);
-  const long long capacity = static_cast<long long>(p.c.max_pages) * p.c.page_size;
-  const int tiles = mapped ? q_tiles(p.max_sq, p.c.batch, p.group, p.c.kv_heads, capacity) : 0;
+  return mapped ? q_tiles(p.max_sq, p.c.batch, p.group, p.c.kv_heads, key_capacity(p)) : 0;
+}
+
+// One attention of all rows over one set of page tables; per_sm: blocks of paged_attn_kernel.
+int launch_rows(const PagedParams& p, const PagedSpace& sp, uint8_t* ws, int sms, int per_sm, cudaStream_t stream) {
+  const int tiles = tiles_of(p);
   if (tiles == 1) return launch_tiles<1>(p, sp, ws, sms, stream);
   if (tiles == 2) return launch_tiles<2>(p, sp, ws, sms, stream);
-  return launch(p.add_o ? paged_attn_kernel<true> : paged_attn_kernel<false>, sms * kPagedPerSm, kPagedWarps * 32, kPagedSmem, stream, p);
+  return launch(p.add_o ? paged_attn_kernel<true> : paged_attn_kernel<false>, sms * per_sm, kPagedWarps * 32, kPagedSmem,
+                stream, p);
 }
 
 int launch_paged(const Fav4PagedArgs& a, int causal, uint8_t* ws, cudaStream_t stream) {
@@ -246,7 +252,7 @@ int launch_paged(const Fav4PagedArgs& a, int causal, uint8_t* ws, cudaStream_t s
   p.causal = causal;
   p.o = static_cast<__nv_bfloat16*>(a.o);
   p.lse = a.lse;
-  if (!a.prefix_pages) return launch_rows(p, sp, ws, sms, stream);
+  if (!a.prefix_pages) return launch_rows(p, sp, ws, sms, kPagedPerSm, stream);
   // every row of the batch against the prefix, as one sequence without a mask, into the workspace in FP32;
   // then the sequences' own keys, joined with it (rows of no sequence are never written)
   PagedParams first = p;
@@ -263,11 +269,16 @@ int launch_paged(const Fav4PagedArgs& a, int causal, uint8_t* ws, cudaStream_t s
   first.part_o = reinterpret_cast<float*>(ws + sp.part + PagedSpace::kPart);
   first.part_ml = reinterpret_cast<float*>(ws + sp.part + PagedSpace::kPart + PagedSpace::kPartO);
   first.arrived += kMaxGrid;
-  rc = launch_rows(first, sp, ws, sms, stream);
+  rc = launch_rows(first, sp, ws, sms, kPagedPerSm, stream);
   if (rc) return rc;
   p.add_o = first.o32;
   p.add_lse = first.lse;
-  return launch_rows(p, sp, ws, sms, stream);
+  // Behind paged_attn_kernel, whose blocks leave the SMs one by one, the own keys take one block per SM while their
+  // tables are not much wider than the prefix's: 8 sequences, 8 heads, of up to 100 keys behind 1000 13.2 us against
+  // 15.3, behind 32768 37.0 against 39.5, 1000 to 4000 behind 32768 52.5 against 54.9; but up to 4000 behind 300 25.1
+  // against 23.3, and behind the tile kernel 64 of up to 2048 behind 32768 51.2 against 45.7.
+  const bool few = tiles_of(first) == 0 && p.c.batch * key_capacity(p) <= 2 * key_capacity(first);
+  return launch_rows(p, sp, ws, sms, few ? 1 : kPagedPerSm, stream);
 }
 
 int forward_paged(const Fav4PagedArgs* a, int causal, void* workspace, size_t bytes, cudaStream_t stream,

@@ -17,10 +17,10 @@
 //   warp 11          the schedule: pieces of work into a small ring that the other warps read
 //
 // Schedule. A unit is (sequence, K/V head, Q tiles of `block_tokens` tokens) and has as many steps as
-// 128-key tiles up to its last visible key. All units lie on one line of steps, with room before each for what
-// it costs beside them, and every block takes an equal stretch of it, so ragged batches, causal chunks and few rows against many keys are balanced
-// alike; the prefix sums of the steps have a closed form, so the line needs no plan and no host. A unit
-// that a boundary cuts leaves (m, l, O) per piece in the workspace, in FP32, and paged_join_kernel adds
+// 128-key tiles up to its last visible key. All units lie on one line of steps, with room before each for
+// what it costs beside them, and every block takes an equal stretch of it, so ragged batches, causal chunks
+// and few rows against many keys are balanced alike; the prefix sums of the steps have a closed form, so the
+// line needs no plan and no host. A unit that a boundary cuts leaves (m, l, O) per piece in the workspace, in FP32, and paged_join_kernel adds
 // them up in key order.
 //
 // Measured with the join: 4096 tokens behind 28672 keys, 8 heads on 2, 498 us (1030 TFLOP/s at the power limit,
