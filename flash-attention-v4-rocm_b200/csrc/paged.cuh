@@ -338,15 +338,14 @@ __device__ __forceinline__ void finish_row(const PagedParams& p, const RowPlace&
   const int64_t lse_at = static_cast<int64_t>(at.head) * p.total_q + at.token;
   if (p.add_o != nullptr) {
     const float other = __ldcg(p.add_lse + lse_at) * 1.4426950408889634f;  // base 2; -inf where that result saw no key
-    const float top = fmaxf(m, other);
-    if (top != -INFINITY) {
-      const float w = exp2f(m - top), x = exp2f(other - top);
-      const float4 b = __ldcg(reinterpret_cast<const float4*>(p.add_o + row * 128 + lane * 4));
-      // where x is 0 the other row is zero
-      acc = make_float4(acc.x * w + b.x * x, acc.y * w + b.y * x, acc.z * w + b.z * x, acc.w * w + b.w * x);
-      l = l * w + x;
-      m = top;
-    }
+    // relative to 0 where neither saw a key: a NaN of either still goes through
+    const float top = fmaxf(m, other), zero = top == -INFINITY ? 0.f : top;
+    const float w = exp2f(m - zero), x = exp2f(other - zero);
+    const float4 b = __ldcg(reinterpret_cast<const float4*>(p.add_o + row * 128 + lane * 4));
+    // where x is 0 the other row is zero
+    acc = make_float4(acc.x * w + b.x * x, acc.y * w + b.y * x, acc.z * w + b.z * x, acc.w * w + b.w * x);
+    l = l * w + x;
+    m = top;
   }
   const float inv = l == 0.f ? 0.f : 1.f / l;  // l is 0 when no key was seen; NaN goes through
   acc = make_float4(acc.x * inv, acc.y * inv, acc.z * inv, acc.w * inv);

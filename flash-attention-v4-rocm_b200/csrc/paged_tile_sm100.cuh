@@ -732,13 +732,12 @@ __global__ void __launch_bounds__(384, 1)
       float a = 1.f, x = 0.f;
       if (live && p.add_o != nullptr) {  // the other result of this row, joined in
         const float other = __ldcg(p.add_lse + lse_at) * 1.4426950408889634f;
-        const float top = fmaxf(m, other);
-        if (top != -INFINITY) {
-          a = exp2f(m - top);
-          x = exp2f(other - top);
-          l = l * a + x;
-          m = top;
-        }
+        // relative to 0 where neither saw a key: a NaN of either still goes through
+        const float top = fmaxf(m, other), zero = top == -INFINITY ? 0.f : top;
+        a = exp2f(m - zero);
+        x = exp2f(other - zero);
+        l = l * a + x;
+        m = top;
       }
       const float inv = l == 0.f ? 0.f : 1.f / l;
       a *= inv;

@@ -527,3 +527,37 @@ def test_results_that_overlap_an_input_are_refused(cuda):
     with pytest.raises(RuntimeError, match="overlap k or v"):
         paged.append(q, both.view(-1)[:3 * 2 * D].view(3, 2, D), v, *cache, cos, sin, out=both[:3])
     paged.attention(both[:3], *cache, 2, out=torch.empty_like(both[:3]))
+
+
+# prefix and own keys on the 16-row kernel; the prefix on the tile kernel; both on it, with one tile and with two
+NAN_BEHIND = [
+    ([1] * 8, [0, 2, 17, 0, 64, 65, 99, 100], 8, 8, 16, 300),
+    ([1] * 40, [0] + [13 * i for i in range(39)], 8, 2, 16, 1500),
+    ([30, 1, 40], [2, 0, 50], 6, 3, 48, 777),
+    ([30, 1, 70], [2, 0, 90], 6, 3, 48, 777),
+    ([300, 260], [5, 0], 8, 2, 64, 1500),
+]
+
+
+@pytest.mark.parametrize("sq,keys,h,hk,page,prefix", NAN_BEHIND)
+def test_nan_query_behind_a_prefix_shows_in_its_rows_only(cuda, sq, keys, h, hk, page, prefix):
+    # rows that see no own key take the prefix's result as it is, NaN included
+    x = Batch(sq, keys, h, hk, page, seed=71, prefix=prefix)
+    first = [int(a) for a in x.cu[:-1]]
+    for t in first:
+        x.q[t, 1] = float("nan")
+    o, lse = attend_shared(x)
+    assert torch.isnan(o[first, 1]).all() and torch.isnan(lse[1, first]).all()
+    o[first, 1], lse[1, first] = 0, 0
+    assert torch.isfinite(o).all() and torch.isfinite(lse).all()
+
+
+@pytest.mark.parametrize("sq,keys,h,hk,page,prefix", NAN_BEHIND)
+def test_nan_of_a_prefix_key_shows_in_every_row_of_its_heads(cuda, sq, keys, h, hk, page, prefix):
+    x = Batch(sq, keys, h, hk, page, seed=72, prefix=prefix)
+    s = prefix // 2
+    x.k_cache[int(x.prefix_pages[s // page]), s % page, 0] = float("nan")
+    o, lse = attend_shared(x)
+    heads = h // hk
+    assert torch.isnan(o[:, :heads]).all() and torch.isnan(lse[:heads]).all()
+    assert torch.isfinite(o[:, heads:]).all() and torch.isfinite(lse[heads:]).all()
