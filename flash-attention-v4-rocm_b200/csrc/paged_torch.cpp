@@ -76,6 +76,10 @@ void no_grad(const char* what, std::initializer_list<const at::Tensor*> tensors)
   for (const at::Tensor* t : tensors)
     TORCH_CHECK(!t->requires_grad(), what, " has no gradient: call it under torch.no_grad(), or detach its inputs");
 }
+// A tensor that was written: an expression that saved it for its backward has to notice.
+void written(const at::Tensor& t) {
+  if (!t.is_inference()) t.unsafeGetTensorImpl()->bump_version();
+}
 // Whether a contiguous result and an input share memory: other blocks still read rows where one writes its own.
 bool overlap(const at::Tensor& out, const at::Tensor& in) {
   if (out.numel() == 0 || in.numel() == 0) return false;
@@ -186,6 +190,9 @@ PyObject* append(PyObject*, PyObject* const* a, Py_ssize_t n) {
   p.heads = fits(heads, "heads");
   p.total_q = fits(tokens, "the number of tokens");
   check_status(fav4_bshd_paged_append(&p, c10::cuda::getCurrentCUDAStream(dev.index())), "paged append");
+  written(tensor_arg(a[3], "k_cache"));
+  written(tensor_arg(a[4], "v_cache"));
+  if (a[12] != Py_None) written(out);
   return THPVariable_Wrap(out);
   END_HANDLE_TH_ERRORS
 }
@@ -254,6 +261,7 @@ PyObject* attend(PyObject*, PyObject* const* a, Py_ssize_t n) {
                                                                                       ws.numel(), stream),
                  "paged attention");
   }
+  if (a[9] != Py_None) written(out);
   if (!with_lse) return THPVariable_Wrap(out);
   PyObject* both = PyTuple_New(2);
   if (!both) throw python_error();

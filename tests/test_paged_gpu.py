@@ -561,3 +561,31 @@ def test_nan_of_a_prefix_key_shows_in_every_row_of_its_heads(cuda, sq, keys, h, 
     heads = h // hk
     assert torch.isnan(o[:, :heads]).all() and torch.isnan(lse[:heads]).all()
     assert torch.isfinite(o[:, heads:]).all() and torch.isfinite(lse[heads:]).all()
+
+
+def test_written_tensors_tell_autograd(cuda):
+    # a tensor that an expression saved for its backward is not overwritten unnoticed
+    x = Batch([2, 1], [50, 40], 8, 2, 16, seed=73)
+    q, k, v, _, cos, sin = do_append(x, 128, False, cuda, fused=False)
+    cache = (x.k_cache, x.v_cache, x.table, x.lens, x.cu)
+    one = torch.ones((), dtype=torch.bfloat16, device=cuda, requires_grad=True)
+
+    def raises(saved, call):
+        loss = (one * saved).sum()
+        call()
+        with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+            loss.backward()
+
+    for saved in (x.k_cache, x.v_cache, x.k_cache[1:]):
+        raises(saved, lambda: paged.append(q, k, v, *cache, cos, sin))
+    out = torch.zeros_like(q)
+    raises(out, lambda: paged.append(q, k, v, *cache, cos, sin, out=out))
+    raises(out, lambda: paged.attention(q, *cache, 2, out=out))
+    versions = [t._version for t in (q, k, v, *cache)]
+    paged.attention(q, *cache, 2)
+    assert versions == [t._version for t in (q, k, v, *cache)]  # what is only read stays as it is
+    with torch.inference_mode():  # tensors without a version
+        a, b = x.k_cache.clone(), x.v_cache.clone()
+        paged.append(q, k, v, a, b, *cache[2:], cos, sin, out=torch.empty_like(q))
+        paged.append(q, k, v, *cache, cos, sin)
+        assert torch.equal(a.view(torch.int16), x.k_cache.view(torch.int16))
