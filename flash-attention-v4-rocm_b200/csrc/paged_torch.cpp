@@ -10,6 +10,7 @@
 #include <Python.h>
 #include <ATen/ATen.h>
 #include <ATen/core/grad_mode.h>
+#include <c10/core/AutogradState.h>
 #include <c10/cuda/CUDAGuard.h>
 #include <c10/cuda/CUDAStream.h>
 #include <cuda_runtime_api.h>
@@ -72,9 +73,12 @@ const void* rows(const at::Tensor& t, const char* name, const at::Device& dev, i
   return t.const_data_ptr();
 }
 void no_grad(const char* what, std::initializer_list<const at::Tensor*> tensors) {
-  if (!at::GradMode::is_enabled()) return;
-  for (const at::Tensor* t : tensors)
-    TORCH_CHECK(!t->requires_grad(), what, " has no gradient: call it under torch.no_grad(), or detach its inputs");
+  if (at::GradMode::is_enabled())
+    for (const at::Tensor* t : tensors)
+      TORCH_CHECK(!t->requires_grad(), what, " has no gradient: call it under torch.no_grad(), or detach its inputs");
+  if (c10::AutogradState::get_tls_state().get_fw_grad_mode())  // torch.no_grad() leaves forward mode on
+    for (const at::Tensor* t : tensors)
+      TORCH_CHECK(!t->_fw_grad(0).defined(), what, " has no gradient, forward-mode neither: unpack its dual inputs");
 }
 // A tensor that was written: an expression that saved it for its backward has to notice.
 void written(const at::Tensor& t) {

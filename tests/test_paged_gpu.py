@@ -589,3 +589,22 @@ def test_written_tensors_tell_autograd(cuda):
         paged.append(q, k, v, a, b, *cache[2:], cos, sin, out=torch.empty_like(q))
         paged.append(q, k, v, *cache, cos, sin)
         assert torch.equal(a.view(torch.int16), x.k_cache.view(torch.int16))
+
+
+def test_inputs_with_a_tangent_are_refused(cuda):
+    # forward-mode derivatives, which torch.no_grad() does not turn off
+    import torch.autograd.forward_ad as fwd
+    x = Batch([2, 1], [50, 40], 8, 2, 16, seed=74)
+    q, k, v, _, cos, sin = do_append(x, 128, False, cuda, fused=False)
+    appends = [q, k, v, x.k_cache, x.v_cache, x.table, x.lens, x.cu, cos, sin]
+    attends = [x.q, x.k_cache, x.v_cache, x.table, x.lens, x.cu, 2]
+    with fwd.dual_level():
+        for call, args, places in ((paged.append, appends, (0, 1, 2, 3, 4, 8, 9)), (paged.attention, attends, (0, 1, 2))):
+            for i in places:
+                dual = [fwd.make_dual(t, torch.ones_like(t)) if j == i else t for j, t in enumerate(args)]
+                with pytest.raises(RuntimeError, match="no gradient"):
+                    call(*dual)
+                with torch.no_grad(), pytest.raises(RuntimeError, match="no gradient"):
+                    call(*dual)
+        paged.attention(*attends)
+    paged.attention(*attends)
