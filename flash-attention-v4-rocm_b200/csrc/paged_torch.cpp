@@ -189,6 +189,8 @@ PyObject* append(PyObject*, PyObject* const* a, Py_ssize_t n) {
     TORCH_CHECK((q.is_contiguous() && out.const_data_ptr() == q.const_data_ptr()) || !overlap(out, q),
                 "out may be q's own memory, but not a part of it");
     TORCH_CHECK(!overlap(out, k) && !overlap(out, v), "out must not overlap k or v");
+    TORCH_CHECK(!overlap(out, tensor_arg(a[3], "k_cache")) && !overlap(out, tensor_arg(a[4], "v_cache")),
+                "out must not overlap the caches");
   }
   p.q_out = out.data_ptr();
   p.heads = fits(heads, "heads");
@@ -249,6 +251,8 @@ PyObject* attend(PyObject*, PyObject* const* a, Py_ssize_t n) {
                 "out must be contiguous bfloat16 of q's shape");
     no_grad("paged attention", {&out});
     TORCH_CHECK(!overlap(out, q), "out must not overlap q");
+    TORCH_CHECK(!overlap(out, tensor_arg(a[1], "k_cache")) && !overlap(out, tensor_arg(a[2], "v_cache")),
+                "out must not overlap the caches");
   }
   p.o = out.data_ptr();
   const bool with_lse = bool_arg(a[10]);

@@ -46,7 +46,8 @@ def append(q, k, v, k_cache, v_cache, page_table, seq_lens, cu_q, cos=None, sin=
     """Writes k and v of the new tokens into their slots and returns q, with q and k rotated by the rows of cos / sin
     (FP32 ``[positions, rotary/2]``) at their positions; ``cos=None`` appends without rotation. q ``[T, H, 128]``, k and
     v ``[T, H_kv, 128]`` may be strided (slices of one projection). ``offsets`` (int32 ``[B]``) shifts a sequence's
-    rotation positions, for keys behind a shared prefix. ``out`` may be q's own memory when q is contiguous."""
+    rotation positions, for keys behind a shared prefix. ``out`` may be q's own memory when q is contiguous, and
+    must not overlap anything else."""
     return load_binding().append(q, k, v, k_cache, v_cache, page_table, seq_lens, cu_q, cos, sin, interleaved, offsets, out)
 
 
@@ -54,7 +55,7 @@ def attention(q, k_cache, v_cache, page_table, seq_lens, cu_q, max_sq: int, *, c
               return_lse=False):
     """O ``[T, H, 128]``, or (O, LSE ``[H, T]``), of packed queries over the pages. ``max_sq`` bounds the new tokens of
     a sequence. Causal is bottom-right: row i of sq sees keys up to ``seq_lens[b] - sq + i``; rows without a key get
-    O = 0 and LSE = -inf. ``out`` must not overlap q. Rows of no sequence, and a sequence's rows past ``max_sq``, are
+    O = 0 and LSE = -inf. ``out`` must not overlap q or the caches. Rows of no sequence, and a sequence's rows past ``max_sq``, are
     not written."""
     return load_binding().attend(q, k_cache, v_cache, page_table, seq_lens, cu_q, max_sq, causal, scale, out, return_lse,
                              None, None)

@@ -347,9 +347,9 @@ int fav4_bshd_paged_append(const Fav4PagedAppendArgs* args, cudaStream_t stream)
  * causal = 1 the rows are a sequence's newest keys: row i of sq sees keys [0,
  * seq_lens[b] - sq + i] (bottom-right, unlike the top-left mask of
  * fav4_bshd_forward; the same where sq = sk). With causal = 0 every row sees
- * every key. o: BF16 [total_q, heads, 128], contiguous; lse: optional FP32
- * [heads, total_q], natural log. A row that sees no key gets O = 0 and LSE =
- * -inf.
+ * every key. o: BF16 [total_q, heads, 128], contiguous, no part of q's memory
+ * or of the cache's; lse: optional FP32 [heads, total_q], natural log. A row that
+ * sees no key gets O = 0 and LSE = -inf.
  *
  * Shared prefix: prefix_len (device int32 [1]) keys at prefix_pages (device int32
  * [max_prefix_pages], pages of the same cache) stand before every sequence's own

@@ -608,3 +608,24 @@ def test_inputs_with_a_tangent_are_refused(cuda):
                     call(*dual)
         paged.attention(*attends)
     paged.attention(*attends)
+
+
+def test_results_that_overlap_the_caches_are_refused(cuda):
+    x = Batch([2, 1], [50, 40], 8, 2, 16, seed=77)
+    q, k, v, _, cos, sin = do_append(x, 128, False, cuda, fused=False)
+    cache = (x.k_cache, x.v_cache, x.table, x.lens, x.cu)
+    for c in (x.k_cache, x.v_cache):
+        rows = c.view(-1)
+        for out in (rows[:q.numel()].view_as(q), rows[-q.numel():].view_as(q)):
+            with pytest.raises(RuntimeError, match="overlap the caches"):
+                paged.attention(q, *cache, 2, out=out)
+            with pytest.raises(RuntimeError, match="overlap the caches"):
+                paged.shared_prefix_attention(q, *cache[:2], x.prefix_pages, x.prefix_len, *cache[2:], 2, out=out)
+            with pytest.raises(RuntimeError, match="overlap the caches"):
+                paged.append(q, k, v, *cache, cos, sin, out=out)
+    pool = torch.zeros(2 * x.k_cache.numel() + q.numel(), dtype=torch.bfloat16, device=cuda)  # neighbours are no overlap
+    n = x.k_cache.numel()
+    k_cache, out, v_cache = (part.view(like.shape) for part, like in
+                             zip(pool.split((n, q.numel(), n)), (x.k_cache, q, x.v_cache)))
+    k_cache.copy_(x.k_cache), v_cache.copy_(x.v_cache)
+    assert torch.equal(paged.attention(q, k_cache, v_cache, *cache[2:], 2, out=out), paged.attention(q, *cache, 2))
