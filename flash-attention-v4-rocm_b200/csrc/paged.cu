@@ -2,7 +2,6 @@
 // layout and launches. Nothing is allocated and the host never synchronises.
 #include <cuda_runtime.h>
 
-#include <algorithm>
 #include <climits>
 #include <cmath>
 #include <cstdint>
@@ -127,29 +126,10 @@ bool paged_valid(const Fav4PagedArgs* a) {
          stride_ok(a->q_token_stride) && stride_ok(a->q_head_stride);
 }
 
-// Q tiles per block for `batch` sequences of at most `tokens` new tokens each behind page tables for `capacity`
-// keys; 0 for paged_attn_kernel. `rows` of a sequence share a K/V head; lengths are not known here.
-//   16-row kernel or tiles. Up to 16 rows the former reads at HBM speed with half the start-up: 32 sequences
-//   of up to 32767 keys take 89 us against 103 with 4 rows, 58 against 62 with 16 (and with 24: 79 against 62).
-//   But the last block of a unit joins its pieces alone, and with few units there are many: with 8 rows, one
-//   unit of 8000 keys 27 us against 17, four units 20 against 17, eight 18 against 19, 64 units of 500 to 1500
-//   keys 15 against 21. With 16 rows 16 units of 100 to 1000 keys 15 against 14, 32 of 8000 34 against 39.
-//   One tile or two. Two tiles read each key half as often and have half the units; one makes smaller pieces and
-//   less padding and has both warpgroups on every step. Long chunks take two: 4096 tokens behind 28672 keys (16384
-//   rows) 502 us against 525, 3 ragged ones of up to 2000 rows 31 against 33, 8 of 1024 rows behind 8000 keys 87
-//   against 93 (but one of 2048 rows behind 8000 35 against 33); and so do prompts that begin their sequence, whose
-//   units have few steps, as tables not much wider than the chunk tell: 4 of 4096 tokens 171 against 183, 8 of 512
-//   rows (8 heads) 23 against 32, 8 of 257 24 against 26. The others take one: 32 of 600 rows behind 1000 keys 49
-//   against 55, 4 of 600 (8 heads) behind 600 32 against 39, 256 rows on 32768 keys 27 against 32.
-int q_tiles(long long tokens, int batch, int group, int kv_heads, long long capacity) {
-  const long long rows = tokens * group, units = static_cast<long long>(batch) * kv_heads;
-  if (group > kBlockM || (rows <= kPagedRows && rows < 2 * units && (rows <= 8 || units >= 32))) return 0;
-  return rows >= 1024 || (rows > kBlockM && capacity < 2 * tokens) ? 2 : 1;
-}
-
 // Workspace: counters first (their place never changes, so that any call may follow any other), then the
 // pieces of units that paged_attn_kernel cuts (a prefixed call's two launches overlap, and have their own),
-// those of paged_tile_kernel, then the first of a prefixed call's two results.
+// those of paged_tile_kernel, then the first of a prefixed call's two results. Sized by the rows alone: a
+// server's batch and tables change from step to step, and its workspace has to do for all of them.
 struct PagedSpace {
   size_t part, tile_o, tile_ml, cut, first_o, first_lse, total;
   static constexpr size_t kCounters = 4096;
@@ -157,13 +137,10 @@ struct PagedSpace {
   static constexpr size_t kPart = kPartO + size_t(2) * kMaxGrid * kPagedRows * 2 * sizeof(float);
 };
 static_assert(2 * kMaxGrid * sizeof(uint32_t) <= PagedSpace::kCounters, "two calls' counters");
+static_assert(kTileRows == kBlockM, "q_tiles counts in the rows of a Q tile");
 static_assert(kMaxSms <= 256, "paged_join_kernel reads one cut unit per thread");
 PagedSpace paged_space(const Fav4PagedArgs& a) {
-  const int group = a.heads / a.cache.kv_heads;
-  const long long page = a.cache.page_size;
-  int tiles = q_tiles(a.max_sq, a.cache.batch, group, a.cache.kv_heads, a.cache.max_pages * page);
-  if (a.prefix_pages)
-    tiles = std::max(tiles, q_tiles(a.total_q, 1, group, a.cache.kv_heads, a.max_prefix_pages * page));
+  const int tiles = q_tiles_bound(a.prefix_pages ? a.total_q : a.max_sq, a.heads);
   PagedSpace s;
   s.part = PagedSpace::kCounters;
   s.tile_o = s.part + (a.prefix_pages ? 2 : 1) * PagedSpace::kPart;

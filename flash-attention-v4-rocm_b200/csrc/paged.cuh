@@ -262,7 +262,6 @@ struct PagedParams {
   float scale_log2;
 };
 
-constexpr int kPagedRows = 16;
 constexpr int kPagedTile = 64;  // keys per tile: one 16-key group per warp
 constexpr int kPagedWarps = 4;
 constexpr int kPagedStages = 3;

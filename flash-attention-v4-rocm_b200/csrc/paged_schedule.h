@@ -1,4 +1,5 @@
-// The arithmetic of the paged attention's schedules, for the kernels and for a host compiler.
+// The arithmetic of the paged attention's schedules and the choice of its kernel, for the kernels, their launches
+// and a host compiler.
 #pragma once
 #include <cstdint>
 
@@ -91,5 +92,33 @@ FAV4_HD int64_t tile_seq_work(const SeqView& s, int causal, int bt) {
 
 // How many of a unit's n steps lie before a boundary `at` places after its first one.
 FAV4_HD int steps_before(int64_t at, int n) { return at <= 0 ? 0 : at >= n ? n : static_cast<int>(at); }
+
+constexpr int kPagedRows = 16;  // rows of a unit of paged_attn_kernel
+constexpr int kTileRows = 128;  // and of a Q tile of paged_tile_kernel
+
+// Q tiles per block for `batch` sequences of at most `tokens` new tokens each behind page tables for `capacity`
+// keys; 0 for paged_attn_kernel. `rows` of a sequence share a K/V head; lengths are not known here.
+//   16-row kernel or tiles. Up to 16 rows the former reads at HBM speed with half the start-up: 32 sequences
+//   of up to 32767 keys take 89 us against 103 with 4 rows, 58 against 62 with 16 (and with 24: 79 against 62).
+//   But the last block of a unit joins its pieces alone, and with few units there are many: with 8 rows, one
+//   unit of 8000 keys 27 us against 17, four units 20 against 17, eight 18 against 19, 64 units of 500 to 1500
+//   keys 15 against 21. With 16 rows 16 units of 100 to 1000 keys 15 against 14, 32 of 8000 34 against 39.
+//   One tile or two. Two tiles read each key half as often and have half the units; one makes smaller pieces and
+//   less padding and has both warpgroups on every step. Long chunks take two: 4096 tokens behind 28672 keys (16384
+//   rows) 502 us against 525, 3 ragged ones of up to 2000 rows 31 against 33, 8 of 1024 rows behind 8000 keys 87
+//   against 93 (but one of 2048 rows behind 8000 35 against 33); and so do prompts that begin their sequence, whose
+//   units have few steps, as tables not much wider than the chunk tell: 4 of 4096 tokens 171 against 183, 8 of 512
+//   rows (8 heads) 23 against 32, 8 of 257 24 against 26. The others take one: 32 of 600 rows behind 1000 keys 49
+//   against 55, 4 of 600 (8 heads) behind 600 32 against 39, 256 rows on 32768 keys 27 against 32.
+inline int q_tiles(long long tokens, int batch, int group, int kv_heads, long long capacity) {
+  const long long rows = tokens * group, units = static_cast<long long>(batch) * kv_heads;
+  if (group > kTileRows || (rows <= kPagedRows && rows < 2 * units && (rows <= 8 || units >= 32))) return 0;
+  return rows >= 1024 || (rows > kTileRows && capacity < 2 * tokens) ? 2 : 1;
+}
+
+// A bound on q_tiles over every batch, K/V head count and page table that `tokens` rows of `heads` can meet.
+inline int q_tiles_bound(long long tokens, int heads) {
+  return tokens * (heads < kTileRows ? heads : kTileRows) > kTileRows ? 2 : 1;
+}
 
 }  // namespace fav4

@@ -379,7 +379,9 @@ struct Fav4PagedArgs {
 typedef struct Fav4PagedArgs Fav4PagedArgs;
 
 /* Workspace of the two calls below (0 on invalid arguments). It depends on heads,
- * max_sq, total_q and whether there is a prefix, not on the lengths. */
+ * max_sq, total_q and whether there is a prefix, and on nothing else: neither on
+ * the lengths nor on batch, kv_heads and the tables. More rows or heads never need
+ * less. */
 size_t fav4_bshd_paged_workspace_bytes(const Fav4PagedArgs* args);
 int fav4_bshd_forward_paged(const Fav4PagedArgs* args, int causal, void* workspace, size_t workspace_bytes,
                             cudaStream_t stream);

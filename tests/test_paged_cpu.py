@@ -172,3 +172,24 @@ def test_fake_refusals(change):
 def test_schema_says_what_is_written():
     schema = str(torch.ops.fav4.paged_append.default._schema)
     assert re.search(r"Tensor\(\w+!\) k_cache, Tensor\(\w+!\) v_cache", schema)
+
+
+SIZES = [(8, 1, 1), (8, 4, 64), (8, 257, 2056), (16, 8, 8), (160, 1, 40), (7, 19, 300)]
+TABLES = [dict(batch=b, kv_heads=hk, page_size=page, max_pages=n)
+          for b in (1, 4, 64, 1000) for hk in (1, 2, 7, 8, 160) for page in (16, 128) for n in (1, 20, 512, 8192)]
+
+
+@pytest.mark.parametrize("prefix", [False, True])
+def test_workspace_depends_on_the_rows_alone(lib, prefix):
+    # a server's batch and tables change from step to step: one workspace does for all of them
+    def need(table, heads, max_sq, total_q, pages=4):
+        more = dict(prefix_pages=A, prefix_len=A, max_prefix_pages=pages) if prefix else {}
+        return lib.fav4_bshd_paged_workspace_bytes(C.byref(paged_args(table, heads=heads, max_sq=max_sq,
+                                                                      total_q=total_q, **more)))
+
+    for heads, max_sq, total_q in SIZES:
+        sizes = {need(t, heads, max_sq, total_q, pages) for t in TABLES if heads % t["kv_heads"] == 0
+                 for pages in (1, 4, 3000)}
+        assert len(sizes) == 1 and min(sizes) > 0, (heads, max_sq, total_q, sizes)
+        for more in ((2 * heads, max_sq, total_q), (heads, max_sq + 1, total_q + 1), (heads, max_sq, 3 * total_q)):
+            assert need(dict(kv_heads=1), *more) >= max(sizes)

@@ -81,3 +81,39 @@ def test_closed_forms(tmp_path):
     r = subprocess.run([str(exe)], capture_output=True, text=True)
     assert r.returncode == 0, (r.returncode, r.stdout)
     assert int(r.stdout) > 100000
+
+
+KERNELS = r"""
+#include <cstdio>
+#include "paged_schedule.h"
+using namespace fav4;
+int main() {
+  const int heads_of[] = {1, 2, 7, 8, 16, 40, 128, 160, 256, 1024}, batches[] = {1, 2, 5, 33, 64, 1000};
+  const long tokens_of[] = {1, 2, 3, 4, 5, 8, 15, 16, 17, 64, 127, 128, 129, 257, 1023, 1024, 5000};
+  const long tables[] = {16, 64, 400, 2048, 8192, 1 << 20};
+  int seen[3] = {0};
+  for (int heads : heads_of)
+    for (int kv = 1; kv <= heads; ++kv) {
+      if (heads % kv) continue;
+      for (long tokens : tokens_of)
+        for (int batch : batches)
+          for (long keys : tables) {
+            const int tiles = q_tiles(tokens, batch, heads / kv, kv, keys);
+            if (tiles < 0 || tiles > q_tiles_bound(tokens, heads)) {
+              printf("heads %d kv %d tokens %ld batch %d keys %ld: %d tiles\n", heads, kv, tokens, batch, keys, tiles);
+              return 1;
+            }
+            ++seen[tiles];
+          }
+    }
+  return seen[0] && seen[1] && seen[2] ? 0 : 2;
+}
+"""
+
+
+def test_workspaces_have_room_for_every_choice_of_kernel(tmp_path):
+    src, exe = tmp_path / "kernels.cpp", tmp_path / "kernels"
+    src.write_text(KERNELS)
+    subprocess.run(["g++", "-O1", "-std=c++17", f"-I{F.PKG_ROOT / 'csrc'}", str(src), "-o", str(exe)], check=True)
+    r = subprocess.run([str(exe)], capture_output=True, text=True)
+    assert r.returncode == 0, (r.returncode, r.stdout)
