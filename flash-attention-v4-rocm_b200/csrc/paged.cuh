@@ -34,10 +34,12 @@ struct PagedCacheView {
   int num_pages, page_size, max_pages, kv_heads, batch;
 };
 
-// A load through L1 (the ordinary case) or past it.
+// A load through L1 (the ordinary case) or past it. Never the non-coherent path: that is for memory which stays as it
+// is for as long as the kernel runs, and these kernels are resident while their predecessor still writes, append's
+// queries before an attention for one.
 template <bool PastL1, typename T>
 __device__ __forceinline__ T load(const T* p) {
-  return PastL1 ? __ldcg(p) : __ldg(p);
+  return PastL1 ? __ldcg(p) : *p;
 }
 
 // Offsets, lengths and rows of sequence b, clamped so that malformed ones can give wrong rows but no access
@@ -97,17 +99,17 @@ __device__ __forceinline__ bool find_sequence(const PagedCacheView& c, const int
   while (hi - lo > 31) {
     const int step = (hi - lo + 31) / 32;
     const int64_t i = lo + static_cast<int64_t>(lane) * step + step - 1;
-    const bool before = i < hi && __ldg(cu + i + 1) <= t;
+    const bool before = i < hi && load<false>(cu + i + 1) <= t;
     lo += __popc(__ballot_sync(0xffffffffu, before)) * step;
     hi = min(hi, lo + step - 1);
   }
   const int i = lo + lane;
   const bool any = i < c.batch;
   AppendSeq s;
-  s.begin = any ? __ldg(cu + i) : 0;
-  s.end = any ? __ldg(cu + i + 1) : 0;
-  s.len = any ? __ldg(c.lens + i) : 0;
-  s.offset = any && offsets != nullptr ? __ldg(offsets + i) : 0;
+  s.begin = any ? load<false>(cu + i) : 0;
+  s.end = any ? load<false>(cu + i + 1) : 0;
+  s.len = any ? load<false>(c.lens + i) : 0;
+  s.offset = any && offsets != nullptr ? load<false>(offsets + i) : 0;
   const int at = __popc(__ballot_sync(0xffffffffu, i < hi && s.end <= t));
   out->b = lo + at;
   out->begin = __shfl_sync(0xffffffffu, s.begin, at);
@@ -174,15 +176,15 @@ __global__ void __launch_bounds__(256) paged_append_kernel(const __grid_constant
     const int64_t row = min(max(at, int64_t(0)), static_cast<int64_t>(p.table_rows) - 1);
     const float4* cp = reinterpret_cast<const float4*>(p.cos_t + row * (p.rotary / 2) + slot * 8);
     const float4* sp = reinterpret_cast<const float4*>(p.sin_t + row * (p.rotary / 2) + slot * 8);
-    cs[0] = __ldg(cp);
-    cs[1] = __ldg(cp + 1);
-    sn[0] = __ldg(sp);
-    sn[1] = __ldg(sp + 1);
+    cs[0] = load<false>(cp);
+    cs[1] = load<false>(cp + 1);
+    sn[0] = load<false>(sp);
+    sn[1] = load<false>(sp + 1);
   }
   int64_t dst_kv = -1;  // a position without a slot (negative, past the table, no such page) is not written
   if (r0 + kAppendRows > p.heads && pos >= 0 && pos < static_cast<int64_t>(p.c.max_pages) * p.c.page_size) {
     const int idx = static_cast<int>(pos) / p.c.page_size;
-    const int page = __ldg(p.c.table + seq.b * p.c.table_stride + idx);
+    const int page = load<false>(p.c.table + seq.b * p.c.table_stride + idx);
     if (page >= 0 && page < p.c.num_pages)
       dst_kv = page * p.c.page_stride + (static_cast<int>(pos) - idx * p.c.page_size) * p.c.token_stride;
   }

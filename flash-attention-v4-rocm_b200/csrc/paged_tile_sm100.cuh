@@ -303,7 +303,7 @@ __global__ void __launch_bounds__(384, 1)
         auto page_of = [&](int j) -> int {
           const int key = (w.tile0 + j) * kTileKeys + lane * R;  // lengths stay well below INT_MAX
           if (lane >= groups || j >= N || key >= w.len) return 0;
-          return min(max(__ldg(table + key / p.c.page_size), 0), p.c.num_pages - 1);
+          return min(max(load<false>(table + key / p.c.page_size), 0), p.c.num_pages - 1);
         };
         int page = page_of(0);
         for (int g = -KA; g < N && ok; ++g) {

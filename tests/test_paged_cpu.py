@@ -193,3 +193,10 @@ def test_workspace_depends_on_the_rows_alone(lib, prefix):
         assert len(sizes) == 1 and min(sizes) > 0, (heads, max_sq, total_q, sizes)
         for more in ((2 * heads, max_sq, total_q), (heads, max_sq + 1, total_q + 1), (heads, max_sq, 3 * total_q)):
             assert need(dict(kv_heads=1), *more) >= max(sizes)
+
+
+def test_kernels_do_not_read_through_the_non_coherent_path():
+    # the kernels are resident while their predecessor writes what they read, so ld.global.nc is not theirs to use
+    for path in (F.PKG_ROOT / "csrc").glob("paged*"):
+        code = re.sub(r"//[^\n]*", "", path.read_text())
+        assert not re.search(r"__ldg\b|\.nc\b|__restrict__", code), path.name
