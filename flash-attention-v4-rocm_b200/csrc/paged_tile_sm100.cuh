@@ -349,6 +349,8 @@ __global__ void __launch_bounds__(384, 1)
         WaitCtl drain{&no_abort, tp.status, tp.wait_limit_ns};
         for (int s = 0; s < Slots; ++s)
           if (st.was_armed(s)) wait_phase(bar(L::kKVFull + s), st.armed_parity(s), drain, kStatusTimeoutDrain);
+        // the parity of the last Q load's phase; with none it is the one that a new barrier has behind it
+        if (!side_v) wait_phase(bar(L::kQFull), st.q_empty(), drain, kStatusTimeoutDrain);
       }
       __syncwarp();
     } else if (warp == 9) {

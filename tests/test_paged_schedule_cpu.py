@@ -1,5 +1,6 @@
 """CPU test of the arithmetic behind the paged attention's schedule (csrc/paged_schedule.h): the closed forms that
 the blocks locate their work with, against sums over every unit."""
+import re
 import subprocess
 from pathlib import Path
 
@@ -117,3 +118,26 @@ def test_workspaces_have_room_for_every_choice_of_kernel(tmp_path):
     subprocess.run(["g++", "-O1", "-std=c++17", f"-I{F.PKG_ROOT / 'csrc'}", str(src), "-o", str(exe)], check=True)
     r = subprocess.run([str(exe)], capture_output=True, text=True)
     assert r.returncode == 0, (r.returncode, r.stdout)
+
+
+def test_an_aborted_block_waits_for_every_copy_it_issued():
+    # a block that gives up must not leave shared memory while a copy is on its way there: each barrier that a TMA
+    # load of the tile kernel signals is waited for where its load warps leave early
+    code = (F.PKG_ROOT / "csrc" / "paged_tile_sm100.cuh").read_text()
+    barriers = set(re.findall(r"tma_load_\dd\([^;]*?(bar\(L::\w+\)|\bfb\b)", code))
+    assert barriers == {"bar(L::kQFull)", "fb"} and "fb = bar(L::kKVFull + ring.stage)" in code
+    abort = code[code.index("if (*abort_flag) {"):]
+    abort = abort[:abort.index("__syncwarp();")]
+    assert re.search(r"wait_phase\(bar\(L::kKVFull \+ s\)", abort) and re.search(r"wait_phase\(bar\(L::kQFull\)", abort)
+
+
+def test_parity_of_the_last_query_load():
+    # LoadState's q_empty is 1 before the first load and turns with each; a barrier's phases complete in order, and
+    # waiting for parity p passes once the phase of that parity has (a new one has parity 1 behind it)
+    for loads in range(6):
+        q_empty = 1
+        for _ in range(loads):
+            q_empty ^= 1
+        for complete in {loads, max(loads - 1, 0)}:
+            passes = (complete - 1) % 2 == q_empty  # the phase before the current one
+            assert passes == (complete == loads)
