@@ -13,6 +13,7 @@ build/fav4_paged_torch.so is the PyTorch binding of the paged cache entries
 from __future__ import annotations
 
 import argparse
+import importlib.metadata
 import importlib.util
 import os
 import shutil
@@ -60,6 +61,18 @@ def _run(cmd, log: Path, name: str, verbose: bool) -> None:
         print(" ".join(cmd))
 
 
+def _torch() -> str | None:
+    """Which torch the binding is compiled against, without importing it; None where there is none."""
+    spec = importlib.util.find_spec("torch")
+    if spec is None:
+        return None
+    try:
+        version = importlib.metadata.version("torch")
+    except importlib.metadata.PackageNotFoundError:  # a source tree on the path
+        version = "?"
+    return f"{version} {spec.origin} python {sys.version.split()[0]}"
+
+
 def binding_command(out: Path) -> list[str]:
     import sysconfig
 
@@ -87,12 +100,15 @@ def build(force: bool = False, verbose: bool = False) -> list[Path]:
             cmd = [nvcc(), *ARCH_FLAGS, *COMMON, "-o", str(out), *[str(CSRC / s) for s in srcs]]
             _run(cmd, BUILD / f"{lib}.ptxas.txt", lib, verbose)
         built.append(out)
-    out = BUILD / BINDING
-    if importlib.util.find_spec("torch") is None:
+    out, stamp, torch_now = BUILD / BINDING, BUILD / f"{BINDING}.torch", _torch()
+    if torch_now is None:
         print(f"{BINDING} is not built: there is no torch here (the C ABI does not need it)", file=sys.stderr)
         return built
-    if force or _stale(out, [BINDING_SRC, *INCLUDE.glob("*.h")]):
+    # it links against torch's C++ ABI: another torch needs another binding
+    other = not stamp.exists() or stamp.read_text() != torch_now
+    if force or other or _stale(out, [BINDING_SRC, *INCLUDE.glob("*.h")]):
         _run(binding_command(out), BUILD / f"{BINDING}.log", BINDING, verbose)
+        stamp.write_text(torch_now)
     return [*built, out]
 
 
