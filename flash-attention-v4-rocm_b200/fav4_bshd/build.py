@@ -62,9 +62,9 @@ def _run(cmd, log: Path, name: str, verbose: bool) -> None:
 
 
 def _torch() -> str | None:
-    """Which torch the binding is compiled against, without importing it; None where there is none."""
+    """Which torch the binding is compiled against, without importing it; None where there is none with CUDA."""
     spec = importlib.util.find_spec("torch")
-    if spec is None:
+    if spec is None or spec.origin is None or not (Path(spec.origin).parent / "lib" / "libc10_cuda.so").exists():
         return None
     try:
         version = importlib.metadata.version("torch")
@@ -102,7 +102,7 @@ def build(force: bool = False, verbose: bool = False) -> list[Path]:
         built.append(out)
     out, stamp, torch_now = BUILD / BINDING, BUILD / f"{BINDING}.torch", _torch()
     if torch_now is None:
-        print(f"{BINDING} is not built: there is no torch here (the C ABI does not need it)", file=sys.stderr)
+        print(f"{BINDING} is not built: there is no torch with CUDA here (the C ABI does not need it)", file=sys.stderr)
         return built
     # it links against torch's C++ ABI: another torch needs another binding
     other = not stamp.exists() or stamp.read_text() != torch_now

@@ -38,3 +38,14 @@ def test_another_torch_needs_another_binding(compiled, monkeypatch):
     compiled.clear()
     B.build()
     assert compiled == []
+
+
+def test_a_torch_without_cuda_gets_no_binding(compiled, monkeypatch, tmp_path, capsys):
+    # the libraries of the C ABI are built all the same
+    import importlib.util
+    (tmp_path / "torch" / "lib").mkdir(parents=True)
+    (tmp_path / "torch" / "__init__.py").touch()
+    cpu_only = importlib.util.spec_from_file_location("torch", tmp_path / "torch" / "__init__.py")
+    monkeypatch.setattr(importlib.util, "find_spec", lambda name: cpu_only)
+    assert [p.name for p in B.build()] == list(B.TARGETS) == compiled
+    assert "not built" in capsys.readouterr().err
