@@ -84,6 +84,12 @@ void no_grad(const char* what, std::initializer_list<const at::Tensor*> tensors)
 void written(const at::Tensor& t) {
   if (!t.is_inference()) t.unsafeGetTensorImpl()->bump_version();
 }
+// Whether two tensors of one shape lie in memory alike; the stride of a single entry says nothing.
+bool same_layout(const at::Tensor& a, const at::Tensor& b) {
+  for (int64_t d = 0; d < a.dim(); ++d)
+    if (a.size(d) > 1 && a.stride(d) != b.stride(d)) return false;
+  return true;
+}
 // Whether a contiguous result and an input share memory: other blocks still read rows where one writes its own.
 bool overlap(const at::Tensor& out, const at::Tensor& in) {
   if (out.numel() == 0 || in.numel() == 0) return false;
@@ -98,7 +104,7 @@ Fav4PagedCache cache_of(PyObject* const* a, const at::Device& dev) {
   const at::Tensor& v = tensor_arg(a[1], "v_cache");
   const at::Tensor& table = tensor_arg(a[2], "page_table");
   const at::Tensor& lens = tensor_arg(a[3], "seq_lens");
-  TORCH_CHECK(k.dim() == 4 && k.size(3) == kHeadDim && v.sizes() == k.sizes() && v.strides() == k.strides(),
+  TORCH_CHECK(k.dim() == 4 && k.size(3) == kHeadDim && v.sizes() == k.sizes() && same_layout(k, v),
               "k_cache and v_cache must be [pages, page_size, kv_heads, 128] of one layout, got ", k.sizes(), " and ",
               v.sizes());
   TORCH_CHECK(k.scalar_type() == at::kBFloat16 && v.scalar_type() == at::kBFloat16 && k.device() == dev &&

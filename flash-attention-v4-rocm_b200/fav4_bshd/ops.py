@@ -202,7 +202,9 @@ def _check_paged(q, k_cache, v_cache, page_table, seq_lens, cu_q):
                  lambda: f"caches must be [pages, page_size, H_kv, {HEAD_DIM}] with page_size a multiple of 16, got "
                          f"{k_cache.shape} and {v_cache.shape}")
     torch._check(all(x.dtype == torch.bfloat16 for x in (q, k_cache, v_cache)), lambda: "q and the caches must be bfloat16")
-    torch._check(k_cache.stride() == v_cache.stride() and k_cache.stride(3) == 1 and q.stride(2) == 1,
+    # the stride of a single entry says nothing
+    torch._check(all(n <= 1 or a == b for n, a, b in zip(k_cache.shape, k_cache.stride(), v_cache.stride()))
+                 and k_cache.stride(3) == 1 and q.stride(2) == 1,
                  lambda: "the caches must have one layout, and every row contiguous elements")
     torch._check(all(x.dtype == torch.int32 for x in (page_table, seq_lens, cu_q)),
                  lambda: "page_table, seq_lens and cu_q must be int32")

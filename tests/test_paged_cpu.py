@@ -200,3 +200,17 @@ def test_kernels_do_not_read_through_the_non_coherent_path():
     for path in (F.PKG_ROOT / "csrc").glob("paged*"):
         code = re.sub(r"//[^\n]*", "", path.read_text())
         assert not re.search(r"__ldg\b|\.nc\b|__restrict__", code), path.name
+
+
+def test_the_stride_of_a_single_head_says_nothing():
+    # one K/V head: storage with the heads inside and outside the pages is the same memory
+    with FakeTensorMode():
+        x = fakes(hk=1)
+        outside = x["cache"].new_empty(20, 1, 16, 128).transpose(1, 2)
+        assert outside.stride() != x["cache"].stride()
+        o, lse = torch.ops.fav4.paged_forward(x["q"], x["cache"], outside, x["table"], x["lens"], x["cu"], 2, True, -1.0)
+        assert o.shape == x["q"].shape
+        two = fakes(hk=2)
+        with pytest.raises(RuntimeError):
+            torch.ops.fav4.paged_forward(two["q"], two["cache"], two["cache"].new_empty(20, 2, 16, 128).transpose(1, 2),
+                                         two["table"], two["lens"], two["cu"], 2, True, -1.0)

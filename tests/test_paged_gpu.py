@@ -629,3 +629,13 @@ def test_results_that_overlap_the_caches_are_refused(cuda):
                              zip(pool.split((n, q.numel(), n)), (x.k_cache, q, x.v_cache)))
     k_cache.copy_(x.k_cache), v_cache.copy_(x.v_cache)
     assert torch.equal(paged.attention(q, k_cache, v_cache, *cache[2:], 2, out=out), paged.attention(q, *cache, 2))
+
+
+def test_the_stride_of_a_single_head_says_nothing(cuda):
+    # one K/V head: storage with the heads inside and outside the pages is the same memory
+    x = Batch([20, 1], [50, 40], 8, 1, 16, seed=78)
+    want = attend(x)
+    x.v_cache = x.v_cache.view(-1, 1, 16, D).transpose(1, 2)
+    assert x.v_cache.stride() != x.k_cache.stride()
+    got = attend(x)
+    assert torch.equal(got[0], want[0]) and torch.equal(got[1], want[1])
