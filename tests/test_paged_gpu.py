@@ -639,3 +639,44 @@ def test_the_stride_of_a_single_head_says_nothing(cuda):
     assert x.v_cache.stride() != x.k_cache.stride()
     got = attend(x)
     assert torch.equal(got[0], want[0]) and torch.equal(got[1], want[1])
+
+
+# a prefix of the 16-row kernel and own tables much wider than it, or wide for the lengths: the own keys of such a
+# call share the SMs with the end of the prefix, each launch with counters and pieces of its own
+WIDE_OWN = [
+    ([1] * 8, [4000 - 531 * i for i in range(8)], 8, 8, 16, 300, 0),
+    ([1] * 8, [0, 3, 1, 40, 64, 65, 99, 100], 8, 8, 16, 1000, 256),
+    ([1, 1], [700, 9000], 4, 4, 32, 2500, 0),
+]
+
+
+@pytest.mark.parametrize("sq,keys,h,hk,page,prefix,gap", WIDE_OWN)
+@pytest.mark.parametrize("causal", [True, False])
+def test_shared_prefix_before_wide_tables(cuda, sq, keys, h, hk, page, prefix, gap, causal):
+    x = Batch(sq, keys, h, hk, page, seed=75, prefix=prefix, gap=gap)
+    ref = x.reference(causal=False)  # one token a sequence sees every key, with the mask or without
+    first = attend_shared(x, causal)
+    check_attention(*first, ref)
+    for _ in range(10):
+        again = attend_shared(x, causal)
+        assert torch.equal(first[0], again[0]) and torch.equal(first[1], again[1])
+
+
+def test_operators_that_write_and_share(cuda):
+    from fav4_bshd import ops  # noqa: F401
+    x = Batch([2, 1], [50, 40], 8, 2, 16, seed=76, prefix=33)
+    x.k_cache.nan_to_num_(0), x.v_cache.nan_to_num_(0)  # the check compares what is not written
+    cos, sin = tables(64, 128)
+    qkv = torch.randn(3, 12, D, device=cuda).bfloat16()
+    q, k, v = qkv.split((8, 2, 2), dim=1)
+    utils = ("test_schema", "test_faketensor")
+    for offsets in (None, torch.tensor([3, 5], dtype=torch.int32, device=cuda)):
+        torch.library.opcheck(torch.ops.fav4.paged_append.default,
+                              (q, k, v, x.k_cache, x.v_cache, x.table, x.lens, x.cu, cos, sin, False, offsets),
+                              test_utils=utils)
+    torch.library.opcheck(torch.ops.fav4.paged_append.default,
+                          (q, k, v, x.k_cache, x.v_cache, x.table, x.lens, x.cu, None, None, False, None),
+                          test_utils=utils)
+    torch.library.opcheck(torch.ops.fav4.shared_prefix_forward.default,
+                          (x.q, x.k_cache, x.v_cache, x.prefix_pages, x.prefix_len, x.table, x.lens, x.cu, 2, True, -1.0),
+                          test_utils=utils)
