@@ -73,8 +73,8 @@ __device__ __forceinline__ SeqView seq_view(const PagedCacheView& c, const int* 
 // Bandwidth: every row (one head of one token, 256 bytes) is read once and written once. A warp takes
 // 8 rows of one token, 8 lanes per row; a lane holds the two 16-byte pieces that contain 8 whole
 // pairs, and because both pairings put pairs 8s..8s+7 into lane s, the lane's slice of cos / sin is
-// the same 32 bytes either way and is loaded once for its rows. 32 x 4096 tokens of 8 + 8 + 8 heads: 253-261 us,
-// 6.2-6.4 TB/s (0.95-0.98 of the copy rate); 128 single tokens: 4.6 us on the device.
+// the same 32 bytes either way and is loaded once for its rows. 32 x 4096 tokens of 8 + 8 + 8 heads: 259 us,
+// 6.2 TB/s (0.95 of the copy rate); 128 single tokens: 4.6 us on the device.
 // ------------------------------------------------------------------------------------------------
 struct AppendParams {
   PagedCacheView c;

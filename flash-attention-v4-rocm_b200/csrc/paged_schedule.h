@@ -80,8 +80,8 @@ FAV4_HD_CALL int64_t units_steps(SeqView s, int causal, int bt, int64_t r) {
 }
 // The line on which the blocks share the work has room for kUnitExtra steps before each unit's own: what a unit
 // costs beside them (its first loads, the end of the pipeline, its rows' ends). Without it a block of many
-// short units ends last: 4 prompts of 4096 tokens 187 us, with 2 153, 3 155, 4 157; 3 ragged chunks 36.1, 30.9,
-// 30.6, 32.8; 8 prompts of 1000 tokens, 8 heads, 56, 55, 50, 52.
+// short units ends last: 4 prompts of 4096 tokens, 8 heads on 2, 199 us, with 2 152, 3 155, 4 155; 3 ragged chunks
+// 37.9, 32.3, 31.4, 33.9; 8 prompts of 1000 tokens, 8 heads, 56, 57, 50, 52.
 constexpr int kUnitExtra = 3;
 FAV4_HD int64_t units_cost(const SeqView& s, int causal, int bt, int64_t r) {
   return units_steps(s, causal, bt, r) + kUnitExtra * r;
@@ -105,9 +105,9 @@ constexpr int kTileRows = 128;  // and of a Q tile of paged_tile_kernel
 //   keys 15 against 21. With 16 rows 16 units of 100 to 1000 keys 15 against 14, 32 of 8000 34 against 39.
 //   One tile or two. Two tiles read each key half as often and have half the units; one makes smaller pieces and
 //   less padding and has both warpgroups on every step. Long chunks take two: 4096 tokens behind 28672 keys (16384
-//   rows) 502 us against 525, 3 ragged ones of up to 2000 rows 31 against 33, 8 of 1024 rows behind 8000 keys 87
+//   rows) 474 us against 504, 3 ragged ones of up to 2000 rows 31 against 33, 8 of 1024 rows behind 8000 keys 87
 //   against 93 (but one of 2048 rows behind 8000 35 against 33); and so do prompts that begin their sequence, whose
-//   units have few steps, as tables not much wider than the chunk tell: 4 of 4096 tokens 171 against 183, 8 of 512
+//   units have few steps, as tables not much wider than the chunk tell: 4 of 4096 tokens 155 against 167, 8 of 512
 //   rows (8 heads) 23 against 32, 8 of 257 24 against 26. The others take one: 32 of 600 rows behind 1000 keys 49
 //   against 55, 4 of 600 (8 heads) behind 600 32 against 39, 256 rows on 32768 keys 27 against 32.
 inline int q_tiles(long long tokens, int batch, int group, int kv_heads, long long capacity) {

@@ -20,10 +20,10 @@
 // 128-key tiles up to its last visible key. All units lie on one line of steps, with room before each for
 // what it costs beside them, and every block takes an equal stretch of it, so ragged batches, causal chunks
 // and few rows against many keys are balanced alike; the prefix sums of the steps have a closed form, so the
-// line needs no plan and no host. A unit that a boundary cuts leaves (m, l, O) per piece in the workspace, in FP32, and paged_join_kernel adds
-// them up in key order.
+// line needs no plan and no host. A unit that a boundary cuts leaves (m, l, O) per piece in the workspace, in FP32,
+// and paged_join_kernel adds them up in key order.
 //
-// Measured with the join: 4096 tokens behind 28672 keys, 8 heads on 2, 498 us (1030 TFLOP/s at the power limit,
+// Measured with the join: 4096 tokens behind 28672 keys, 8 heads on 2, 489 us (1055 TFLOP/s at the power limit,
 // 1310 in the kernel alone at 1965 MHz), where neither the tensor pipe (54 %) nor MUFU (57 %) is full and the
 // round trip softmax -> P V -> S -> softmax bounds; 16 sequences of 3 to 7 tokens, 71 MB of keys, 25 us, 10 of them
 // at HBM speed between a start of 6, an epilogue and the join.
@@ -770,7 +770,7 @@ __global__ void __launch_bounds__(384, 1)
         if (p.o == nullptr) continue;
         if constexpr (QTiles == 1) {
           // eight lanes write 128 bytes of one row, instead of 32 lanes 16 bytes of as many: 4 prompts of 4096
-          // tokens 178 -> 165 us with one Q tile per block; with two, whose other tile hides the stores, 154 -> 156
+          // tokens 173 -> 167 us with one Q tile per block; with two, whose other tile hides the stores, 155 -> 157
           transpose_pieces(pieces16, lane);
 #pragma unroll
           for (int k = 0; k < 8; ++k) {

@@ -300,7 +300,8 @@ int fav4_bshd_forward_host(const Fav4Args* args, const Fav4HostOut* outs, int n_
  * int32; seq_lens[b] counts every key, this call's new ones included. Lengths
  * are clamped to [0, max_pages * page_size] and page numbers to the cache:
  * malformed ones give wrong rows, never an access outside the arrays. Slots past
- * a sequence's end may hold anything, NaN included. */
+ * a sequence's end may hold anything, NaN included; a masked value within it is
+ * multiplied by 0, so there a NaN or an infinity can show. */
 struct Fav4PagedCache {
   void *k, *v;
   const int* page_table;
